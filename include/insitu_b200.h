@@ -311,6 +311,84 @@ int ivf_pq_encode(const void* d_x, int x_is_u8, long long n, int d, const int* d
                   const int* d_assign, const float* d_codebook, int M, unsigned char* d_codes, void* stream);
 
 /* ======================================================================
+ * Scalar-quantised rows (new): floating rows kept at 8 or 4 bits a value
+ * with fp32 scales, written to slots, read back, and scored by 8-bit products.
+ * Beside the residual PQ above (ivf_pq_encode), whose codes need a trained
+ * codebook, and the exact uint8 rows (ivf_u8_load), which must be whole numbers.
+ *
+ * A store of `capacity` rows is two device arrays of the caller's:
+ *   codes   row s at d_codes + s * ldc bytes: int8 [d] (bits = 8), or two
+ *           codes a byte, the even one in the low half (bits = 4; the last
+ *           high half of an odd d is 0)
+ *   scales  fp32, row s at d_scales + s * lds: one scale per group of `group`
+ *           consecutive values (a multiple of 16; the last group may be
+ *           shorter), or one for the row (group = 0)
+ * With L = 127 (bits 8) or 7 (bits 4):
+ *   scale = fp32(max |x| over the group / L)
+ *   code  = x / scale rounded to the nearest whole number, ties to even, in
+ *           [-L, L]; 0 where the scale is 0
+ *   value = code * scale, rounded once to the type it is read in
+ * A group with a NaN or an infinity has that as its scale and reads as NaN.
+ * No operator here has a gradient.
+ *
+ * Device pointers of the current device; work is queued on `stream` (a
+ * cudaStream_t of that device, NULL = legacy default stream) and the calls
+ * neither allocate nor synchronise, so they may be captured in a graph.
+ * Arrays of floating values are aligned to their type, d_slots to 8 bytes;
+ * 16-byte aligned rows are fastest.  An output must not overlap an input.  Two calls that write one
+ * store (or use one d_claim or d_work) must be ordered.  Failures are
+ * reported through ivf_global_last_error().
+ * ====================================================================== */
+/* types of floating rows */
+#define IVF_SQ_F32 0
+#define IVF_SQ_F16 1
+#define IVF_SQ_BF16 2
+/* most values a row may have */
+#define IVF_SQ_MAX_D 1048576
+/* writes of at most this many rows need no claim table */
+#define IVF_SQ_SCAN_ROWS 512
+/* largest k of the 8-bit products: 2^17 - 1 products of 128 * 128 fit in 32 bits */
+#define IVF_SQ_MAX_K 131071
+/*
+ * Row i of d_x [n, d] (x_type, rows ldx values apart) is quantised into slot
+ * d_slots[i] (NULL: slot i, then n <= capacity).  A row whose slot is outside
+ * [0, capacity) is left out; of rows with one slot the last stays; slots that no row names
+ * are left as they were.  d_claim int32 [capacity] is scratch of any contents,
+ * needed for more than IVF_SQ_SCAN_ROWS rows with slots (else it may be NULL).  n < 2^31.
+ */
+int ivf_sq_write(const void* d_x, int x_type, long long n, int d, long long ldx, const long long* d_slots, int bits,
+                 int group, void* d_codes, long long ldc, float* d_scales, long long lds, long long capacity,
+                 int* d_claim, void* stream);
+/* d_out [n, d] (out_type, rows ldo values apart): the values of slot
+ * d_slots[i] (NULL: slot i, then n <= capacity); a slot outside [0, capacity) reads as zeros */
+int ivf_sq_read(const void* d_codes, long long ldc, const float* d_scales, long long lds, long long capacity,
+                int bits, int group, const long long* d_slots, long long n, int d, void* d_out, int out_type,
+                long long ldo, void* stream);
+/*
+ * 8-bit product with a scale per token (row of a) and per channel (row of b):
+ *   out[i, j] = float(sum_t a[i, t] * b[j, t]) * a_scale[i] * b_scale[j] + bias[j]
+ * a [m, k], b [n, k] int8 (any value), rows lda and ldb bytes apart; scales
+ * and bias (may be NULL) fp32, dense; out [m, n] of out_type, rows ldo values
+ * apart.  The sum is exact (1 <= k <= IVF_SQ_MAX_K); the rest is fp32, rounded
+ * once to out_type.  m, n < 2^31.
+ */
+int ivf_sq_matmul(const int8_t* d_a, long long lda, const float* d_a_scale, long long m, const int8_t* d_b,
+                  long long ldb, const float* d_b_scale, long long n, int k, const float* d_bias, void* d_out,
+                  int out_type, long long ldo, void* stream);
+/*
+ * Scores of floating tokens against n rows of an 8-bit store with one scale a row: d_x [m, d]
+ * (x_type, rows ldx values apart) is quantised as ivf_sq_write does (bits 8,
+ * group 0), then multiplied as by ivf_sq_matmul, with equal results.
+ * d_scales dense [n].  d_work: scratch of ivf_sq_scores_work(m, d) bytes,
+ * 16-byte aligned.
+ */
+int ivf_sq_scores(const void* d_x, int x_type, long long ldx, long long m, const int8_t* d_codes, long long ldc,
+                  const float* d_scales, long long n, int d, const float* d_bias, void* d_out, int out_type,
+                  long long ldo, void* d_work, size_t work_bytes, void* stream);
+/* bytes of d_work that ivf_sq_scores needs (0 for sizes that it refuses) */
+size_t ivf_sq_scores_work(long long m, int d);
+
+/* ======================================================================
  * Update overlay (new: runner-internal in the reference,
  * updates/pq_update.cu:396-494, 975-1055)
  * ====================================================================== */

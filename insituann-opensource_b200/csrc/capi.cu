@@ -1434,6 +1434,162 @@ int ivf_pq_encode(const void* d_x, int x_is_u8, long long n, int d, const int* d
     });
 }
 
+// ---------------------------------------------------------------------------
+// scalar-quantised rows
+// ---------------------------------------------------------------------------
+namespace {
+// require() without building a message that is not needed: these calls are short
+void need(bool ok, const char* msg, const char* what = nullptr) {
+    if (!ok) fail(IVF_EINVAL, what ? std::string(what) + ": " + msg : std::string(msg));
+}
+// what write, read and scores ask of a store and of floating rows
+void sq_check_store(const void* codes, long long ldc, const float* scales, long long lds, long long capacity, int d,
+                    int bits, int group) {
+    need(bits == 8 || bits == 4, "bits must be 8 or 4");
+    need(d >= 1 && d <= IVF_SQ_MAX_D, "need 1 <= d <= IVF_SQ_MAX_D");
+    need(group == 0 || (group > 0 && group % 16 == 0), "group must be 0 or a multiple of 16");
+    need(capacity >= 0 && capacity < (1ll << 40), "need 0 <= capacity < 2^40");
+    need(ldc >= (d * (long long)bits + 7) / 8 && ldc < (1ll << 32), "ldc is below a row's bytes (or above 2^32)");
+    need(lds >= (group ? (d + group - 1) / group : 1) && lds < (1ll << 32),
+            "lds is below a row's number of scales (or above 2^32)");
+    need(capacity == 0 || (codes && scales), "null pointer");
+    need(reinterpret_cast<uintptr_t>(scales) % 4 == 0, "scales must be 4-byte aligned");
+}
+void sq_check_rows(const void* x, int type, long long n, int d, long long ld, const char* what) {
+    need(type == IVF_SQ_F32 || type == IVF_SQ_F16 || type == IVF_SQ_BF16, "unknown type", what);
+    need(n >= 0 && n < 2147483647ll, "need 0 <= rows < 2^31 - 1", what);
+    need(ld >= d && ld < (1ll << 40), "rows overlap (their distance is below their width)", what);
+    need(n == 0 || x, "null pointer", what);
+    need(reinterpret_cast<uintptr_t>(x) % (type == IVF_SQ_F32 ? 4 : 2) == 0, "not aligned", what);
+}
+SqMatmul sq_check_product(const int8_t* b, long long ldb, const float* b_scale, long long m, long long n, int k,
+                          const float* bias, void* out, int out_type, long long ldo) {
+    need(k >= 1 && k <= IVF_SQ_MAX_K, "need 1 <= k <= IVF_SQ_MAX_K");
+    need(n >= 0 && n < 2147483647ll, "need 0 <= n < 2^31 - 1");
+    sq_check_rows(n ? out : nullptr, out_type, n ? m : 0, (int)std::min<long long>(n, 2147483647ll), ldo, "out");
+    need(ldb >= k && ldb < (1ll << 32), "rows of b overlap (their distance is below k)");
+    need(n == 0 || (b && b_scale), "null pointer");
+    need(reinterpret_cast<uintptr_t>(b_scale) % 4 == 0 && reinterpret_cast<uintptr_t>(bias) % 4 == 0,
+            "scales and bias must be 4-byte aligned");
+    SqMatmul p{};
+    p.m = m;
+    p.b = b;
+    p.b_scale = b_scale;
+    p.n = n;
+    p.ldb = ldb;
+    p.k = k;
+    p.bias = bias;
+    p.out = out;
+    p.ldo = ldo;
+    return p;
+}
+// row stride of the quantised tokens in ivf_sq_scores' scratch
+long long sq_work_ld(int d) { return (d + 15ll) / 16 * 16; }
+}  // namespace
+
+int ivf_sq_write(const void* d_x, int x_type, long long n, int d, long long ldx, const long long* d_slots, int bits,
+                 int group, void* d_codes, long long ldc, float* d_scales, long long lds, long long capacity,
+                 int* d_claim, void* stream) {
+    return guarded(nullptr, [&] {
+        sq_check_store(d_codes, ldc, d_scales, lds, capacity, d, bits, group);
+        sq_check_rows(d_x, x_type, n, d, ldx, "x");
+        need(d_slots || n <= capacity, "more rows than slots");
+        need(reinterpret_cast<uintptr_t>(d_slots) % 8 == 0, "slots must be 8-byte aligned");
+        need(!d_slots || n <= IVF_SQ_SCAN_ROWS || d_claim || capacity == 0,
+                "more than IVF_SQ_SCAN_ROWS rows with slots need d_claim");
+        need(reinterpret_cast<uintptr_t>(d_claim) % 4 == 0, "d_claim must be 4-byte aligned");
+        if (capacity == 0) return;
+        SqWrite p{};
+        p.x = d_x;
+        p.n = n;
+        p.ldx = ldx;
+        p.d = d;
+        p.slots = d_slots;
+        p.group = std::min(group, d) == d ? 0 : group;
+        p.codes = static_cast<uint8_t*>(d_codes);
+        p.scales = d_scales;
+        p.ldc = ldc;
+        p.lds = lds;
+        p.capacity = capacity;
+        p.claim = d_claim;
+        ck(sq_write(p, x_type, bits, static_cast<cudaStream_t>(stream)), "sq_write");
+    });
+}
+
+int ivf_sq_read(const void* d_codes, long long ldc, const float* d_scales, long long lds, long long capacity,
+                int bits, int group, const long long* d_slots, long long n, int d, void* d_out, int out_type,
+                long long ldo, void* stream) {
+    return guarded(nullptr, [&] {
+        sq_check_store(d_codes, ldc, d_scales, lds, capacity, d, bits, group);
+        sq_check_rows(d_out, out_type, n, d, ldo, "out");
+        need(d_slots || n <= capacity, "more rows than slots");
+        need(reinterpret_cast<uintptr_t>(d_slots) % 8 == 0, "slots must be 8-byte aligned");
+        SqRead p{};
+        p.codes = static_cast<const uint8_t*>(d_codes);
+        p.scales = d_scales;
+        p.ldc = ldc;
+        p.lds = lds;
+        p.capacity = capacity;
+        p.group = std::min(group, d) == d ? 0 : group;
+        p.slots = d_slots;
+        p.n = n;
+        p.d = d;
+        p.out = d_out;
+        p.ldo = ldo;
+        ck(sq_read(p, out_type, bits, static_cast<cudaStream_t>(stream)), "sq_read");
+    });
+}
+
+int ivf_sq_matmul(const int8_t* d_a, long long lda, const float* d_a_scale, long long m, const int8_t* d_b,
+                  long long ldb, const float* d_b_scale, long long n, int k, const float* d_bias, void* d_out,
+                  int out_type, long long ldo, void* stream) {
+    return guarded(nullptr, [&] {
+        need(m >= 0 && m < 2147483647ll, "need 0 <= m < 2^31 - 1");
+        SqMatmul p = sq_check_product(d_b, ldb, d_b_scale, m, n, k, d_bias, d_out, out_type, ldo);
+        need(lda >= k && lda < (1ll << 32), "rows of a overlap (their distance is below k)");
+        need(m == 0 || (d_a && d_a_scale), "null pointer");
+        need(reinterpret_cast<uintptr_t>(d_a_scale) % 4 == 0, "scales and bias must be 4-byte aligned");
+        p.a = d_a;
+        p.a_scale = d_a_scale;
+        p.lda = lda;
+        if (m == 0 || n == 0) return;
+        ck(sq_matmul(p, out_type, static_cast<cudaStream_t>(stream)), "sq_matmul");
+    });
+}
+
+size_t ivf_sq_scores_work(long long m, int d) {
+    if (m < 0 || m >= 2147483647ll || d < 1 || d > IVF_SQ_MAX_K) return 0;
+    return (size_t)m * (size_t)(sq_work_ld(d) + 4) + 16;
+}
+
+int ivf_sq_scores(const void* d_x, int x_type, long long ldx, long long m, const int8_t* d_codes, long long ldc,
+                  const float* d_scales, long long n, int d, const float* d_bias, void* d_out, int out_type,
+                  long long ldo, void* d_work, size_t work_bytes, void* stream) {
+    return guarded(nullptr, [&] {
+        need(d >= 1 && d <= IVF_SQ_MAX_K, "need 1 <= d <= IVF_SQ_MAX_K");
+        sq_check_rows(d_x, x_type, m, d, ldx, "x");
+        SqMatmul p = sq_check_product(d_codes, ldc, d_scales, m, n, d, d_bias, d_out, out_type, ldo);
+        need(work_bytes >= ivf_sq_scores_work(m, d) && d_work, "d_work is smaller than ivf_sq_scores_work(m, d)");
+        need(reinterpret_cast<uintptr_t>(d_work) % 16 == 0, "d_work must be 16-byte aligned");
+        if (m == 0 || n == 0) return;
+        SqWrite w{};
+        w.x = d_x;
+        w.n = m;
+        w.ldx = ldx;
+        w.d = d;
+        w.codes = static_cast<uint8_t*>(d_work);
+        w.ldc = sq_work_ld(d);
+        w.scales = reinterpret_cast<float*>(w.codes + (size_t)m * w.ldc);
+        w.lds = 1;
+        w.capacity = m;
+        ck(sq_write(w, x_type, 8, static_cast<cudaStream_t>(stream)), "sq_scores (quantise)");
+        p.a = reinterpret_cast<const int8_t*>(w.codes);
+        p.a_scale = w.scales;
+        p.lda = w.ldc;
+        ck(sq_matmul(p, out_type, static_cast<cudaStream_t>(stream)), "sq_scores (product)");
+    });
+}
+
 int ivf_set_shard(void* idx_ctx, int nlist_global, const int* local_to_global, const long long* key_offsets) {
     IndexCtx* x = nullptr;
     try {

@@ -218,4 +218,50 @@ cudaError_t pq_merge_shards(const uint64_t* adc_main, const uint64_t* exact_main
                             int nq, int k, int exact_is_int, int32_t* out_ids, float* out_dist,
                             cudaStream_t st);
 
+// ---- scalar-quantised rows (sq.cu, sq_mm.cu) -------------------------------
+constexpr int kSqF32 = 0, kSqF16 = 1, kSqBF16 = 2;   // IVF_SQ_* of the C ABI
+// calls of up to this many rows look for a later row with the same slot
+// themselves (each row compares the slots after its own); longer ones go
+// through the claim table
+constexpr int kSqScanRows = 512;
+constexpr int kSqAll = 0, kSqScan = 1, kSqClaim = 2;
+struct SqWrite {
+    const void* x;               // [n, d] rows, ldx values apart
+    int64_t n, ldx;
+    int d;
+    const long long* slots;      // [n]; null: row i goes to slot i
+    int group, groups;           // values per scale (0: the row), scales per row (set by sq_write)
+    uint8_t* codes;              // [capacity], ldc bytes apart
+    float* scales;               // [capacity, groups], lds apart
+    int64_t ldc, lds, capacity;
+    int* claim;                  // [capacity] scratch, needed above kSqScanRows rows with slots
+    int dedup;                   // set by sq_write
+};
+cudaError_t sq_write(SqWrite p, int type, int bits, cudaStream_t st);
+struct SqRead {
+    const uint8_t* codes;
+    const float* scales;
+    int64_t ldc, lds, capacity;
+    int group, groups;           // as in SqWrite
+    const long long* slots;      // [n]; null: row i reads slot i
+    int64_t n;
+    int d;
+    void* out;                   // [n, d], ldo values apart
+    int64_t ldo;
+};
+cudaError_t sq_read(SqRead p, int type, int bits, cudaStream_t st);
+struct SqMatmul {
+    const int8_t* a;             // [m, k] tokens, lda apart
+    const float* a_scale;        // [m]
+    int64_t m, lda;
+    const int8_t* b;             // [n, k] channels, ldb apart
+    const float* b_scale;        // [n]
+    int64_t n, ldb;
+    int k;
+    const float* bias;           // [n] or null
+    void* out;                   // [m, n], ldo apart
+    int64_t ldo;
+};
+cudaError_t sq_matmul(const SqMatmul& p, int out_type, cudaStream_t st);
+
 }  // namespace isb

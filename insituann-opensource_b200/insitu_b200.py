@@ -45,6 +45,7 @@ EXPORTS = [
     "ivf_last_error", "ivf_global_last_error",
     "ivf_kernel_launches", "ivf_batch_profile", "ivf_batch_stage_ms", "ivf_u8_search_noalloc",
     "ivf_load_centroids", "ivf_assign", "ivf_build_reorder", "ivf_kmeans_update", "ivf_pq_train", "ivf_pq_encode",
+    "ivf_sq_write", "ivf_sq_read", "ivf_sq_matmul", "ivf_sq_scores", "ivf_sq_scores_work",
     "ivf_read_centroids", "ivf_read_assign", "ivf_read_codebook", "ivf_read_codes", "ivf_read_u8bin",
     "ivf_read_fbin", "ivf_read_gt", "ivf_write_centroids", "ivf_write_assign", "ivf_write_codebook",
     "ivf_write_codes", "ivf_pq_load_files", "ivf_pq_insert",
@@ -118,6 +119,11 @@ _SIGS = {
     "ivf_kmeans_update": ([vp, i32, i64, i32, vp, i32, vp, vp], i32),
     "ivf_pq_train": ([vp, i32, i64, i32, vp, vp, i32, i32, vp, vp], i32),
     "ivf_pq_encode": ([vp, i32, i64, i32, vp, vp, vp, vp, i32, vp, vp], i32),
+    "ivf_sq_write": ([vp, i32, i64, i32, i64, vp, i32, i32, vp, i64, vp, i64, i64, vp, vp], i32),
+    "ivf_sq_read": ([vp, i64, vp, i64, i64, i32, i32, vp, i64, i32, vp, i32, i64, vp], i32),
+    "ivf_sq_matmul": ([vp, i64, vp, i64, vp, i64, vp, i64, i32, vp, vp, i32, i64, vp], i32),
+    "ivf_sq_scores": ([vp, i32, i64, i64, vp, i64, vp, i64, i32, vp, vp, i32, i64, vp, C.c_size_t, vp], i32),
+    "ivf_sq_scores_work": ([i64, i32], C.c_size_t),
     "ivf_read_centroids": ([C.c_char_p, vp, i64, vp, vp], i64),
     "ivf_read_assign": ([C.c_char_p, vp, i64, vp], i64),
     "ivf_read_codebook": ([C.c_char_p, vp, i64, vp, vp, vp], i64),
@@ -644,6 +650,239 @@ class Builder:
                                          assign.data_ptr(), codebook.data_ptr(), M, codes.data_ptr(),
                                          self._stream()))
         return codes
+
+
+def _sq_rc(L, rc):
+    if rc != IVF_OK:
+        raise InsituError(rc, L.ivf_global_last_error().decode())
+
+
+def _sq_type(dtype):
+    """IVF_SQ_* of a torch dtype."""
+    import torch
+
+    t = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(dtype)
+    if t is None:
+        raise ValueError(f"scalar-quantised rows are read and written as float32, float16 or bfloat16, not {dtype}")
+    return t
+
+
+def _sq_need(ok, msg):
+    if not ok:
+        raise ValueError(msg)
+
+
+def _sq_2d(t, name, device=None):
+    """(tensor with unit steps inside its rows, distance between rows) of a 2-D device tensor"""
+    _sq_need(t.dim() == 2, f"{name} must be 2-D, got shape {tuple(t.shape)}")
+    _sq_need(t.is_cuda, f"{name} must be a CUDA tensor")
+    _sq_need(device is None or t.device == device, f"{name} is on {t.device}, not on {device}")
+    n, d = t.shape
+    if (d > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < d):
+        t = t.contiguous()
+    return t, (t.stride(0) if n > 1 else max(d, t.stride(0)))
+
+
+def _sq_1d(t, name, n, dtype, device):
+    import torch
+
+    _sq_need(t.dim() == 1 and t.shape[0] == n, f"{name} must have shape ({n},), got {tuple(t.shape)}")
+    _sq_need(t.is_cuda and t.device == device, f"{name} must be on {device}")
+    if dtype is torch.int64:
+        _sq_need(t.dtype in (torch.int64, torch.int32), f"{name} must be int64 or int32, got {t.dtype}")
+        t = t.to(dtype)
+    _sq_need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
+    return t.contiguous()
+
+
+def _sq_out(out, shape, dtype, device):
+    """(output tensor, distance between its rows)"""
+    import torch
+
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=device)
+        return out, max(shape[1], 1)
+    _sq_need(tuple(out.shape) == tuple(shape), f"out must have shape {tuple(shape)}, got {tuple(out.shape)}")
+    _sq_need(out.dtype == dtype and out.device == device, f"out must be {dtype} on {device}")
+    _sq_need((shape[1] <= 1 or out.stride(1) == 1) and (shape[0] <= 1 or out.stride(0) >= shape[1]),
+             "out must have unit steps inside its rows, and rows that do not overlap")
+    return out, (out.stride(0) if shape[0] > 1 else max(shape[1], out.stride(0)))
+
+
+def _sq_call(fn, device, *args):
+    """fn(*args, stream) with the tensors' device current, on torch's current stream of that device"""
+    import torch
+
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _sq_bias(bias, n, device):
+    import torch
+
+    return None if bias is None else _sq_1d(bias, "bias", n, torch.float32, device)
+
+
+def sq_matmul(a, a_scale, b, b_scale, bias=None, dtype=None, out=None):
+    """8-bit matrix product with a scale per token and per channel (ivf_sq_matmul):
+
+        out[i, j] = (sum_t a[i, t] * b[j, t]) * a_scale[i] * b_scale[j] + bias[j]
+
+    a int8 [m, k] and b int8 [n, k] (rows at any distance; 16-byte aligned rows
+    are fastest), a_scale fp32 [m], b_scale fp32 [n], bias fp32 [n] or None.
+    dtype: torch.float32 (default), float16 or bfloat16.  The sum is exact, the
+    rest fp32 and rounded once.  Runs on the current torch stream of the
+    tensors' device; no gradient flows."""
+    import torch
+
+    L = load_library()
+    _sq_need(a.dtype == torch.int8 and b.dtype == torch.int8, "a and b must be int8")
+    a, lda = _sq_2d(a, "a")
+    dev = a.device
+    b, ldb = _sq_2d(b, "b", dev)
+    (m, k), n = a.shape, b.shape[0]
+    _sq_need(b.shape[1] == k, f"a has rows of {k} values, b of {b.shape[1]}")
+    a_scale = _sq_1d(a_scale, "a_scale", m, torch.float32, dev)
+    b_scale = _sq_1d(b_scale, "b_scale", n, torch.float32, dev)
+    bias = _sq_bias(bias, n, dev)
+    dtype = dtype or (torch.float32 if out is None else out.dtype)
+    t = _sq_type(dtype)
+    out, ldo = _sq_out(out, (m, n), dtype, dev)
+    _sq_rc(L, _sq_call(L.ivf_sq_matmul, dev, a.data_ptr(), lda, a_scale.data_ptr(), m, b.data_ptr(), ldb,
+                       b_scale.data_ptr(), n, k, _p(bias), out.data_ptr(), t, ldo))
+    return out
+
+
+class SQRows:
+    """A store of scalar-quantised rows: `capacity` slots of `d` values at 8 or 4
+    bits with one fp32 scale per `group` values (0: per row), in device tensors.
+
+    ``write`` quantises floating rows into slots (online inserts, a cache that
+    grows), ``read`` turns slots back into values, ``scores`` multiplies floating
+    queries with every row by 8-bit products.  With L = 127 (8 bits) or 7 (4
+    bits): scale = max |x| / L, code = round-half-even(x / scale), value = code *
+    scale.  A group with a NaN or an infinity reads back as NaN.
+
+    ``codes``  int8 [capacity, >= d] or uint8 [capacity, >= ceil(d / 2)] (two
+    codes a byte, the even one in the low half); ``scales`` fp32 [capacity,
+    groups].  Slots never written are zeros.
+
+    Work runs on the current torch stream of the store's device; two writes of
+    one store must be ordered.  No gradient flows through any call."""
+
+    def __init__(self, capacity: int, d: int, bits: int = 8, group: int = 0, device=None):
+        import torch
+
+        load_library(require_device=True)
+        _sq_need(bits in (8, 4), "bits must be 8 or 4")
+        _sq_need(capacity >= 0 and d >= 1 and group >= 0, "need capacity >= 0, d >= 1, group >= 0")
+        ld = ((d * bits + 7) // 8 + 15) // 16 * 16
+        device = torch.device("cuda" if device is None else device)
+        codes = torch.zeros((capacity, ld), dtype=torch.int8 if bits == 8 else torch.uint8, device=device)
+        scales = torch.zeros((capacity, -(-d // group) if group else 1), dtype=torch.float32, device=device)
+        self._adopt(codes, scales, d, bits, group)
+
+    @classmethod
+    def from_arrays(cls, codes, scales, d: int, bits: int = 8, group: int = 0) -> "SQRows":
+        """a store over existing device tensors (as ``codes`` and ``scales`` above), which it shares"""
+        load_library(require_device=True)
+        rows = cls.__new__(cls)
+        rows._adopt(codes, scales, d, bits, group)
+        return rows
+
+    def _adopt(self, codes, scales, d, bits, group):
+        import torch
+
+        _sq_need(bits in (8, 4), "bits must be 8 or 4")
+        _sq_need(1 <= d <= 1 << 20, "need 1 <= d <= 2^20")
+        _sq_need(group >= 0 and group % 16 == 0, "group must be 0 or a multiple of 16")
+        _sq_need(codes.dim() == 2 and scales.dim() == 2 and codes.shape[0] == scales.shape[0],
+                 "codes and scales must be 2-D with a row per slot")
+        _sq_need(codes.is_cuda and scales.device == codes.device, "codes and scales must be on one CUDA device")
+        _sq_need(codes.dtype == (torch.int8 if bits == 8 else torch.uint8) and scales.dtype == torch.float32,
+                 "codes must be int8 (8 bits) or uint8 (4 bits), scales float32")
+        n = codes.shape[0]
+        _sq_need(codes.shape[1] >= (d * bits + 7) // 8, "codes rows are shorter than d values")
+        _sq_need(scales.shape[1] == (-(-d // group) if group else 1), "scales must have a column per group")
+        for t in (codes, scales):
+            _sq_need((t.shape[1] <= 1 or t.stride(1) == 1) and (n <= 1 or t.stride(0) >= t.shape[1]),
+                     "codes and scales must have unit steps inside their rows, and rows that do not overlap")
+        self.L = load_library()
+        self.codes, self.scales = codes, scales
+        self.capacity, self.d, self.bits, self.group = n, d, bits, group
+        self.device = codes.device
+        self._ldc = codes.stride(0) if n > 1 else max(codes.shape[1], codes.stride(0))
+        self._lds = scales.stride(0) if n > 1 else max(scales.shape[1], scales.stride(0))
+
+    def _slots(self, slots, n):
+        import torch
+
+        if slots is None:
+            _sq_need(n <= self.capacity, f"{n} rows for {self.capacity} slots")
+            return None
+        return _sq_1d(slots, "slots", n, torch.int64, self.device)
+
+    def write(self, x, slots=None):
+        """rows x [n, d] (fp32, fp16 or bf16) into slots [n] (None: slots 0 .. n - 1).
+
+        A row whose slot is outside the store is left out; of rows with one
+        slot the last stays; other slots are left as they were."""
+        import torch
+
+        x, ldx = _sq_2d(x, "x", self.device)
+        n, d = x.shape
+        _sq_need(d == self.d, f"x has rows of {d} values, the store of {self.d}")
+        t = _sq_type(x.dtype)
+        slots = self._slots(slots, n)
+        claim = None
+        if slots is not None and n > 512:
+            claim = torch.empty(max(self.capacity, 1), dtype=torch.int32, device=self.device)
+        _sq_rc(self.L, _sq_call(self.L.ivf_sq_write, self.device, x.data_ptr(), t, n, d, ldx, _p(slots), self.bits,
+                                self.group, self.codes.data_ptr(), self._ldc, self.scales.data_ptr(), self._lds,
+                                self.capacity, _p(claim)))
+        return self
+
+    def read(self, slots=None, dtype=None, out=None):
+        """values [n, d] of slots [n] (None: every slot); a slot outside the store reads as zeros.
+        dtype: torch.float32 (default), float16 or bfloat16."""
+        import torch
+
+        dtype = dtype or (torch.float32 if out is None else out.dtype)
+        t = _sq_type(dtype)
+        n = self.capacity if slots is None else slots.shape[0]
+        slots = self._slots(slots, n)
+        out, ldo = _sq_out(out, (n, self.d), dtype, self.device)
+        _sq_rc(self.L, _sq_call(self.L.ivf_sq_read, self.device, self.codes.data_ptr(), self._ldc,
+                                self.scales.data_ptr(), self._lds, self.capacity, self.bits, self.group, _p(slots), n,
+                                self.d, out.data_ptr(), t, ldo))
+        return out
+
+    def scores(self, x, bias=None, dtype=None, out=None):
+        """[m, capacity] products of floating rows x [m, d] with every row of an
+        8-bit store with one scale a row (group 0): x is quantised one scale a
+        row as ``write`` does it, then multiplied as by sq_matmul.  bias fp32
+        [capacity] or None; dtype of the scores: torch.float32 (default),
+        float16 or bfloat16."""
+        import torch
+
+        _sq_need(self.bits == 8 and self.scales.shape[1] == 1, "scores needs an 8-bit store with one scale a row")
+        _sq_need(self._lds == 1 or self.capacity <= 1, "scores needs dense scales")
+        x, ldx = _sq_2d(x, "x", self.device)
+        m, d = x.shape
+        _sq_need(d == self.d, f"x has rows of {d} values, the store of {self.d}")
+        t = _sq_type(x.dtype)
+        bias = _sq_bias(bias, self.capacity, self.device)
+        dtype = dtype or (torch.float32 if out is None else out.dtype)
+        to = _sq_type(dtype)
+        out, ldo = _sq_out(out, (m, self.capacity), dtype, self.device)
+        need = self.L.ivf_sq_scores_work(m, d)
+        work = torch.empty(need, dtype=torch.uint8, device=self.device)
+        _sq_rc(self.L, _sq_call(self.L.ivf_sq_scores, self.device, x.data_ptr(), t, ldx, m, self.codes.data_ptr(),
+                                self._ldc, self.scales.data_ptr(), self.capacity, d, _p(bias), out.data_ptr(), to,
+                                ldo, work.data_ptr(), need))
+        return out
 
 
 class CoarseTiming(C.Structure):
