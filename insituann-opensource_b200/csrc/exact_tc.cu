@@ -502,6 +502,8 @@ EncodeTiledFn encode_fn() {
 
 }  // namespace
 
+void* encode_tiled_entry() { return reinterpret_cast<void*>(encode_fn()); }
+
 bool exact_tc_usable(int d, int k) { return (d == 128 || d == 256) && k > 0 && k <= kTKMax; }
 
 cudaError_t exact_tc_map(const uint8_t* rows, int64_t n, int d, void* map_out) {

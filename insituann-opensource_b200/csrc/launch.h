@@ -35,6 +35,8 @@ constexpr int kGroupQueries = 4;
 // ---- exact uint8 search on the tensor cores (exact_tc.cu) ------------------
 // d in {128, 256}, 0 < k <= 16
 bool exact_tc_usable(int d, int k);
+// cuTensorMapEncodeTiled of the loaded driver (null when it has none)
+void* encode_tiled_entry();
 // the tensor map (128 bytes, 64-byte aligned) over rows [n, d] of an exact index
 cudaError_t exact_tc_map(const uint8_t* rows, int64_t n, int d, void* map_out);
 // the grouped exact search (groups of up to 127 queries, wl.gq = 127) with q.x
