@@ -139,6 +139,8 @@ _SIGS = {
     "ivf_pq_insert": ([vp, vp, i32, vp, i64], i32),
 }
 
+_SQ_SCAN_ROWS = 512      # IVF_SQ_SCAN_ROWS
+
 STAGES = ("route", "worklist", "scan", "select", "rerank")
 
 _lib = None
@@ -652,18 +654,23 @@ class Builder:
         return codes
 
 
-def _sq_rc(L, rc):
-    if rc != IVF_OK:
-        raise InsituError(rc, L.ivf_global_last_error().decode())
+def _sq_fail(rc):
+    raise InsituError(rc, load_library().ivf_global_last_error().decode())
+
+
+_SQ_TYPES: dict = {}     # torch dtype -> IVF_SQ_*
 
 
 def _sq_type(dtype):
     """IVF_SQ_* of a torch dtype."""
-    import torch
-
-    t = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(dtype)
+    t = _SQ_TYPES.get(dtype)
     if t is None:
-        raise ValueError(f"scalar-quantised rows are read and written as float32, float16 or bfloat16, not {dtype}")
+        import torch
+
+        _SQ_TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        t = _SQ_TYPES.get(dtype)
+        if t is None:
+            raise ValueError(f"scalar-quantised rows are read and written as float32, float16 or bfloat16, not {dtype}")
     return t
 
 
@@ -672,41 +679,51 @@ def _sq_need(ok, msg):
         raise ValueError(msg)
 
 
+# The checks below are on the path of calls of a few microseconds: messages are
+# made only where a check fails.
+
 def _sq_2d(t, name, device=None):
-    """(tensor with unit steps inside its rows, distance between rows) of a 2-D device tensor"""
-    _sq_need(t.dim() == 2, f"{name} must be 2-D, got shape {tuple(t.shape)}")
-    _sq_need(t.is_cuda, f"{name} must be a CUDA tensor")
-    _sq_need(device is None or t.device == device, f"{name} is on {t.device}, not on {device}")
+    """(tensor with unit steps inside its rows, distance between rows, rows, row width) of a 2-D device tensor"""
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-D, got shape {tuple(t.shape)}")
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise ValueError(f"{name} is on {t.device}, not on {device or 'a CUDA device'}")
     n, d = t.shape
-    if (d > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < d):
+    ld, step = t.stride()
+    if (step != 1 and d > 1) or (ld < d and n > 1):
         t = t.contiguous()
-    return t, (t.stride(0) if n > 1 else max(d, t.stride(0)))
+        ld = d
+    return t, (ld if n > 1 and ld > 0 else max(d, 1)), n, d
 
 
 def _sq_1d(t, name, n, dtype, device):
-    import torch
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} must have shape ({n},), got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.dtype != dtype:
+        import torch
 
-    _sq_need(t.dim() == 1 and t.shape[0] == n, f"{name} must have shape ({n},), got {tuple(t.shape)}")
-    _sq_need(t.is_cuda and t.device == device, f"{name} must be on {device}")
-    if dtype is torch.int64:
-        _sq_need(t.dtype in (torch.int64, torch.int32), f"{name} must be int64 or int32, got {t.dtype}")
+        if dtype != torch.int64 or t.dtype != torch.int32:
+            raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
         t = t.to(dtype)
-    _sq_need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
     return t.contiguous()
 
 
-def _sq_out(out, shape, dtype, device):
+def _sq_out(out, n, d, dtype, device):
     """(output tensor, distance between its rows)"""
-    import torch
-
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
-        return out, max(shape[1], 1)
-    _sq_need(tuple(out.shape) == tuple(shape), f"out must have shape {tuple(shape)}, got {tuple(out.shape)}")
-    _sq_need(out.dtype == dtype and out.device == device, f"out must be {dtype} on {device}")
-    _sq_need((shape[1] <= 1 or out.stride(1) == 1) and (shape[0] <= 1 or out.stride(0) >= shape[1]),
-             "out must have unit steps inside its rows, and rows that do not overlap")
-    return out, (out.stride(0) if shape[0] > 1 else max(shape[1], out.stride(0)))
+        import torch
+
+        return torch.empty((n, d), dtype=dtype, device=device), d or 1
+    if tuple(out.shape) != (n, d):
+        raise ValueError(f"out must have shape {(n, d)}, got {tuple(out.shape)}")
+    if out.dtype != dtype or out.device != device:
+        raise ValueError(f"out must be {dtype} on {device}")
+    ld, step = out.stride()
+    if (d > 1 and step != 1) or (n > 1 and ld < d):
+        raise ValueError("out must have unit steps inside its rows, and rows that do not overlap")
+    return out, (ld if n > 1 and ld > 0 else max(d, 1))
 
 
 def _sq_call(fn, device, *args):
@@ -715,14 +732,11 @@ def _sq_call(fn, device, *args):
 
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
-            return fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    return fn(*args, torch.cuda.current_stream(device).cuda_stream)
-
-
-def _sq_bias(bias, n, device):
-    import torch
-
-    return None if bias is None else _sq_1d(bias, "bias", n, torch.float32, device)
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc != IVF_OK:
+        _sq_fail(rc)
 
 
 def sq_matmul(a, a_scale, b, b_scale, bias=None, dtype=None, out=None):
@@ -738,20 +752,22 @@ def sq_matmul(a, a_scale, b, b_scale, bias=None, dtype=None, out=None):
     import torch
 
     L = load_library()
-    _sq_need(a.dtype == torch.int8 and b.dtype == torch.int8, "a and b must be int8")
-    a, lda = _sq_2d(a, "a")
+    if a.dtype != torch.int8 or b.dtype != torch.int8:
+        raise ValueError("a and b must be int8")
+    a, lda, m, k = _sq_2d(a, "a")
     dev = a.device
-    b, ldb = _sq_2d(b, "b", dev)
-    (m, k), n = a.shape, b.shape[0]
-    _sq_need(b.shape[1] == k, f"a has rows of {k} values, b of {b.shape[1]}")
+    b, ldb, n, kb = _sq_2d(b, "b", dev)
+    if k != kb:
+        raise ValueError(f"a has rows of {k} values, b of {kb}")
     a_scale = _sq_1d(a_scale, "a_scale", m, torch.float32, dev)
     b_scale = _sq_1d(b_scale, "b_scale", n, torch.float32, dev)
-    bias = _sq_bias(bias, n, dev)
+    if bias is not None:
+        bias = _sq_1d(bias, "bias", n, torch.float32, dev)
     dtype = dtype or (torch.float32 if out is None else out.dtype)
     t = _sq_type(dtype)
-    out, ldo = _sq_out(out, (m, n), dtype, dev)
-    _sq_rc(L, _sq_call(L.ivf_sq_matmul, dev, a.data_ptr(), lda, a_scale.data_ptr(), m, b.data_ptr(), ldb,
-                       b_scale.data_ptr(), n, k, _p(bias), out.data_ptr(), t, ldo))
+    out, ldo = _sq_out(out, m, n, dtype, dev)
+    _sq_call(L.ivf_sq_matmul, dev, a.data_ptr(), lda, a_scale.data_ptr(), m, b.data_ptr(), ldb, b_scale.data_ptr(),
+             n, k, None if bias is None else bias.data_ptr(), out.data_ptr(), t, ldo)
     return out
 
 
@@ -810,38 +826,52 @@ class SQRows:
             _sq_need((t.shape[1] <= 1 or t.stride(1) == 1) and (n <= 1 or t.stride(0) >= t.shape[1]),
                      "codes and scales must have unit steps inside their rows, and rows that do not overlap")
         self.L = load_library()
-        self.codes, self.scales = codes, scales
+        self._codes, self._scales = codes, scales
         self.capacity, self.d, self.bits, self.group = n, d, bits, group
         self.device = codes.device
         self._ldc = codes.stride(0) if n > 1 else max(codes.shape[1], codes.stride(0))
         self._lds = scales.stride(0) if n > 1 else max(scales.shape[1], scales.stride(0))
+        self._groups = scales.shape[1]
+
+    @property
+    def codes(self):
+        return self._codes
+
+    @property
+    def scales(self):
+        return self._scales
 
     def _slots(self, slots, n):
         import torch
 
         if slots is None:
-            _sq_need(n <= self.capacity, f"{n} rows for {self.capacity} slots")
+            if n > self.capacity:
+                raise ValueError(f"{n} rows for {self.capacity} slots")
             return None
         return _sq_1d(slots, "slots", n, torch.int64, self.device)
+
+    def _rows(self, x):
+        """(x with unit steps inside its rows, distance between rows, rows, type) of floating rows as wide as the store's"""
+        x, ldx, n, d = _sq_2d(x, "x", self.device)
+        if d != self.d:
+            raise ValueError(f"x has rows of {d} values, the store of {self.d}")
+        return x, ldx, n, _sq_type(x.dtype)
 
     def write(self, x, slots=None):
         """rows x [n, d] (fp32, fp16 or bf16) into slots [n] (None: slots 0 .. n - 1).
 
         A row whose slot is outside the store is left out; of rows with one
         slot the last stays; other slots are left as they were."""
-        import torch
-
-        x, ldx = _sq_2d(x, "x", self.device)
-        n, d = x.shape
-        _sq_need(d == self.d, f"x has rows of {d} values, the store of {self.d}")
-        t = _sq_type(x.dtype)
+        x, ldx, n, t = self._rows(x)
         slots = self._slots(slots, n)
         claim = None
-        if slots is not None and n > 512:
+        if slots is not None and n > _SQ_SCAN_ROWS:
+            import torch
+
             claim = torch.empty(max(self.capacity, 1), dtype=torch.int32, device=self.device)
-        _sq_rc(self.L, _sq_call(self.L.ivf_sq_write, self.device, x.data_ptr(), t, n, d, ldx, _p(slots), self.bits,
-                                self.group, self.codes.data_ptr(), self._ldc, self.scales.data_ptr(), self._lds,
-                                self.capacity, _p(claim)))
+        _sq_call(self.L.ivf_sq_write, self.device, x.data_ptr(), t, n, self.d, ldx,
+                 None if slots is None else slots.data_ptr(), self.bits, self.group, self._codes.data_ptr(), self._ldc,
+                 self._scales.data_ptr(), self._lds, self.capacity, None if claim is None else claim.data_ptr())
         return self
 
     def read(self, slots=None, dtype=None, out=None):
@@ -853,10 +883,10 @@ class SQRows:
         t = _sq_type(dtype)
         n = self.capacity if slots is None else slots.shape[0]
         slots = self._slots(slots, n)
-        out, ldo = _sq_out(out, (n, self.d), dtype, self.device)
-        _sq_rc(self.L, _sq_call(self.L.ivf_sq_read, self.device, self.codes.data_ptr(), self._ldc,
-                                self.scales.data_ptr(), self._lds, self.capacity, self.bits, self.group, _p(slots), n,
-                                self.d, out.data_ptr(), t, ldo))
+        out, ldo = _sq_out(out, n, self.d, dtype, self.device)
+        _sq_call(self.L.ivf_sq_read, self.device, self._codes.data_ptr(), self._ldc, self._scales.data_ptr(), self._lds,
+                 self.capacity, self.bits, self.group, None if slots is None else slots.data_ptr(), n, self.d,
+                 out.data_ptr(), t, ldo)
         return out
 
     def scores(self, x, bias=None, dtype=None, out=None):
@@ -867,21 +897,21 @@ class SQRows:
         float16 or bfloat16."""
         import torch
 
-        _sq_need(self.bits == 8 and self.scales.shape[1] == 1, "scores needs an 8-bit store with one scale a row")
-        _sq_need(self._lds == 1 or self.capacity <= 1, "scores needs dense scales")
-        x, ldx = _sq_2d(x, "x", self.device)
-        m, d = x.shape
-        _sq_need(d == self.d, f"x has rows of {d} values, the store of {self.d}")
-        t = _sq_type(x.dtype)
-        bias = _sq_bias(bias, self.capacity, self.device)
+        if self.bits != 8 or self._groups != 1:
+            raise ValueError("scores needs an 8-bit store with one scale a row")
+        if self._lds != 1 and self.capacity > 1:
+            raise ValueError("scores needs dense scales")
+        x, ldx, m, t = self._rows(x)
+        if bias is not None:
+            bias = _sq_1d(bias, "bias", self.capacity, torch.float32, self.device)
         dtype = dtype or (torch.float32 if out is None else out.dtype)
         to = _sq_type(dtype)
-        out, ldo = _sq_out(out, (m, self.capacity), dtype, self.device)
-        need = self.L.ivf_sq_scores_work(m, d)
+        out, ldo = _sq_out(out, m, self.capacity, dtype, self.device)
+        need = self.L.ivf_sq_scores_work(m, self.d)
         work = torch.empty(need, dtype=torch.uint8, device=self.device)
-        _sq_rc(self.L, _sq_call(self.L.ivf_sq_scores, self.device, x.data_ptr(), t, ldx, m, self.codes.data_ptr(),
-                                self._ldc, self.scales.data_ptr(), self.capacity, d, _p(bias), out.data_ptr(), to,
-                                ldo, work.data_ptr(), need))
+        _sq_call(self.L.ivf_sq_scores, self.device, x.data_ptr(), t, ldx, m, self._codes.data_ptr(), self._ldc,
+                 self._scales.data_ptr(), self.capacity, self.d, None if bias is None else bias.data_ptr(), out.data_ptr(),
+                 to, ldo, work.data_ptr(), need)
         return out
 
 
