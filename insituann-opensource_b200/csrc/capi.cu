@@ -1448,7 +1448,7 @@ void sq_check_store(const void* codes, long long ldc, const float* scales, long 
     need(bits == 8 || bits == 4, "bits must be 8 or 4");
     need(d >= 1 && d <= IVF_SQ_MAX_D, "need 1 <= d <= IVF_SQ_MAX_D");
     need(group == 0 || (group > 0 && group % 16 == 0), "group must be 0 or a multiple of 16");
-    need(capacity >= 0 && capacity < (1ll << 40), "need 0 <= capacity < 2^40");
+    need(capacity >= 0 && capacity < 2147483647ll, "need 0 <= capacity < 2^31 - 1");
     need(ldc >= (d * (long long)bits + 7) / 8 && ldc < (1ll << 32), "ldc is below a row's bytes (or above 2^32)");
     need(lds >= (group ? (d + group - 1) / group : 1) && lds < (1ll << 32),
             "lds is below a row's number of scales (or above 2^32)");
@@ -1458,7 +1458,7 @@ void sq_check_store(const void* codes, long long ldc, const float* scales, long 
 void sq_check_rows(const void* x, int type, long long n, int d, long long ld, const char* what) {
     need(type == IVF_SQ_F32 || type == IVF_SQ_F16 || type == IVF_SQ_BF16, "unknown type", what);
     need(n >= 0 && n < 2147483647ll, "need 0 <= rows < 2^31 - 1", what);
-    need(ld >= d && ld < (1ll << 40), "rows overlap (their distance is below their width)", what);
+    need(ld >= d && ld < (1ll << 32), "rows overlap (their distance is below their width), or are 2^32 apart", what);
     need(n == 0 || x, "null pointer", what);
     need(reinterpret_cast<uintptr_t>(x) % (type == IVF_SQ_F32 ? 4 : 2) == 0, "not aligned", what);
 }
@@ -1501,16 +1501,16 @@ int ivf_sq_write(const void* d_x, int x_type, long long n, int d, long long ldx,
         if (capacity == 0) return;
         SqWrite p{};
         p.x = d_x;
-        p.n = n;
-        p.ldx = ldx;
+        p.n = (uint32_t)n;
+        p.ldx = (uint32_t)ldx;
         p.d = d;
         p.slots = d_slots;
         p.group = std::min(group, d) == d ? 0 : group;
         p.codes = static_cast<uint8_t*>(d_codes);
         p.scales = d_scales;
-        p.ldc = ldc;
-        p.lds = lds;
-        p.capacity = capacity;
+        p.ldc = (uint32_t)ldc;
+        p.lds = (uint32_t)lds;
+        p.capacity = (uint32_t)capacity;
         p.claim = d_claim;
         ck(sq_write(p, x_type, bits, static_cast<cudaStream_t>(stream)), "sq_write");
     });
@@ -1527,15 +1527,15 @@ int ivf_sq_read(const void* d_codes, long long ldc, const float* d_scales, long 
         SqRead p{};
         p.codes = static_cast<const uint8_t*>(d_codes);
         p.scales = d_scales;
-        p.ldc = ldc;
-        p.lds = lds;
-        p.capacity = capacity;
+        p.ldc = (uint32_t)ldc;
+        p.lds = (uint32_t)lds;
+        p.capacity = (uint32_t)capacity;
         p.group = std::min(group, d) == d ? 0 : group;
         p.slots = d_slots;
-        p.n = n;
+        p.n = (uint32_t)n;
         p.d = d;
         p.out = d_out;
-        p.ldo = ldo;
+        p.ldo = (uint32_t)ldo;
         ck(sq_read(p, out_type, bits, static_cast<cudaStream_t>(stream)), "sq_read");
     });
 }
@@ -1574,14 +1574,14 @@ int ivf_sq_scores(const void* d_x, int x_type, long long ldx, long long m, const
         if (m == 0 || n == 0) return;
         SqWrite w{};
         w.x = d_x;
-        w.n = m;
-        w.ldx = ldx;
+        w.n = (uint32_t)m;
+        w.ldx = (uint32_t)ldx;
         w.d = d;
         w.codes = static_cast<uint8_t*>(d_work);
-        w.ldc = sq_work_ld(d);
+        w.ldc = (uint32_t)sq_work_ld(d);
         w.scales = reinterpret_cast<float*>(w.codes + (size_t)m * w.ldc);
         w.lds = 1;
-        w.capacity = m;
+        w.capacity = (uint32_t)m;
         ck(sq_write(w, x_type, 8, static_cast<cudaStream_t>(stream)), "sq_scores (quantise)");
         p.a = reinterpret_cast<const int8_t*>(w.codes);
         p.a_scale = w.scales;

@@ -227,15 +227,17 @@ constexpr int kSqF32 = 0, kSqF16 = 1, kSqBF16 = 2;   // IVF_SQ_* of the C ABI
 // through the claim table
 constexpr int kSqScanRows = 512;
 constexpr int kSqAll = 0, kSqScan = 1, kSqClaim = 2;
+// rows, slots and distances between rows are below 2^31 / 2^32, so that an
+// address is one 32 x 32 -> 64-bit multiply-add
 struct SqWrite {
     const void* x;               // [n, d] rows, ldx values apart
-    int64_t n, ldx;
+    uint32_t n, ldx;
     int d;
     const long long* slots;      // [n]; null: row i goes to slot i
     int group, groups;           // values per scale (0: the row), scales per row (set by sq_write)
     uint8_t* codes;              // [capacity], ldc bytes apart
     float* scales;               // [capacity, groups], lds apart
-    int64_t ldc, lds, capacity;
+    uint32_t ldc, lds, capacity;
     int* claim;                  // [capacity] scratch, needed above kSqScanRows rows with slots
     int dedup;                   // set by sq_write
 };
@@ -243,13 +245,13 @@ cudaError_t sq_write(SqWrite p, int type, int bits, cudaStream_t st);
 struct SqRead {
     const uint8_t* codes;
     const float* scales;
-    int64_t ldc, lds, capacity;
+    uint32_t ldc, lds, capacity;
     int group, groups;           // as in SqWrite
     const long long* slots;      // [n]; null: row i reads slot i
-    int64_t n;
+    uint32_t n, ldo;
     int d;
     void* out;                   // [n, d], ldo values apart
-    int64_t ldo;
+    bool once;                   // set by sq_read
 };
 cudaError_t sq_read(SqRead p, int type, int bits, cudaStream_t st);
 struct SqMatmul {

@@ -17,163 +17,266 @@ __device__ __forceinline__ void sq_round(float v, float& o) { o = v; }
 __device__ __forceinline__ void sq_round(float v, __half& o) { o = __float2half_rn(v); }
 __device__ __forceinline__ void sq_round(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 
-// values per chunk: 16 bytes of the floating type, or the fewest that fill a byte of codes
+// Values per chunk: 16 bytes of the floating type where rows are 16-byte aligned
+// and a whole number of chunks long (VEC), else the fewest that fill a byte of
+// codes.  With VEC a chunk is inside its group or outside, so nothing below handles a part of one.
 template <typename T, int BITS, bool VEC>
 __host__ __device__ constexpr int sq_chunk() {
     return VEC ? 16 / (int)sizeof(T) : 8 / BITS;
 }
 
 // item = row * parts + part
-__device__ __forceinline__ void sq_split(int64_t item, int parts, int64_t& row, int& part) {
+__device__ __forceinline__ void sq_split(uint64_t item, int parts, uint32_t& row, int& part) {
     if (parts == 1) {
-        row = item;
+        row = (uint32_t)item;
         part = 0;
-    } else if (item < (int64_t(1) << 32)) {
-        const uint32_t r = (uint32_t)item / (uint32_t)parts;
-        row = r;
-        part = (int)((uint32_t)item - r * (uint32_t)parts);
+    } else if (item >> 32 == 0) {
+        row = (uint32_t)item / (uint32_t)parts;
+        part = (int)((uint32_t)item - row * (uint32_t)parts);
     } else {
-        row = item / parts;
-        part = (int)(item - row * parts);
+        row = (uint32_t)(item / (uint32_t)parts);
+        part = (int)(item - (uint64_t)row * (uint32_t)parts);
     }
 }
 
+// two fp32 operations in one instruction, each rounded as its scalar form
+__device__ __forceinline__ float2 sq_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+        " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 sq_add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+        " add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 sq_mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+        " mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// ---- floating chunks, kept as they were read (half the registers of fp32 for
+// the 16-bit types) ----
+template <typename T, int E>
+struct SqRaw {
+    static constexpr int kWords = (E * (int)sizeof(T) + 3) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+        else {
+            const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+            T t;
+            memcpy(&t, &h, 2);
+            return sq_float(t);
+        }
+    }
+    // raises `top` (bit patterns of |x|, two 16-bit halves apart or one 32-bit) by this chunk's
+    __device__ __forceinline__ void top(uint32_t& t) const {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i)
+            t = sizeof(T) == 4 ? max(t, w[i] & 0x7fffffffu) : __vmaxu2(t, w[i] & 0x7fff7fffu);
+    }
+};
+
 // values e0 .. e0 + E - 1 of a group of `width` values, 0 past its end
 template <typename T, bool VEC, int E>
-__device__ __forceinline__ void sq_load(const T* __restrict__ x, int e0, int width, float (&v)[E]) {
-    if (VEC && e0 + E <= width) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(x + e0);
-        T t[16 / sizeof(T)];
-        memcpy(t, &raw, 16);
+__device__ __forceinline__ SqRaw<T, E> sq_load(const T* __restrict__ x, int e0, int width) {
+    SqRaw<T, E> r;
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = sq_float(t[e]);
+    for (int i = 0; i < SqRaw<T, E>::kWords; ++i) r.w[i] = 0;
+    if constexpr (VEC) {
+        if (e0 < width) {
+            const uint4 v = *reinterpret_cast<const uint4*>(x + e0);
+            memcpy(r.w, &v, sizeof(r.w));
+        }
     } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = e0 + e < width ? sq_float(x[e0 + e]) : 0.f;
+        for (int e = 0; e < E; ++e)
+            if (e0 + e < width) {
+                if constexpr (sizeof(T) == 4) r.w[e] = reinterpret_cast<const uint32_t*>(x)[e0 + e];
+                else r.w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(x)[e0 + e] << (16 * (e & 1));
+            }
+    }
+    return r;
+}
+
+// |x| as fp32 bits from the bit pattern that SqRaw::top raised (halves joined).
+// The maximum is taken over bit patterns: there NaN > infinity > every number.
+template <typename T>
+__device__ __forceinline__ float sq_top(uint32_t t) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(t);
+    else {
+        const uint16_t h = (uint16_t)max(t >> 16, t & 0xffffu);
+        T v;
+        memcpy(&v, &h, 2);
+        return sq_float(v);
     }
 }
 
 struct SqScale {
     float scale;   // as stored
     float inv;     // 1 / scale rounded; 0 where every code is 0 (scale 0, infinite or NaN)
-    float half;    // scale / 2
+    float half;    // a remainder of at least this asks for the slow quotient
 };
 
-// the scale of a group from the bits of its largest |x|.  The maximum is taken
-// over bit patterns: there NaN > infinity > every number.
+// Scales below 2^-100 (where half a step or 1 / scale leaves fp32's range) always take the slow quotient.
 template <int BITS>
-__device__ __forceinline__ SqScale sq_scale(uint32_t top) {
+__device__ __forceinline__ SqScale sq_scale(float top) {
     SqScale s;
-    s.scale = __fdiv_rn(__uint_as_float(top), BITS == 8 ? 127.f : 7.f);
-    const bool none = !(s.scale > 0.f && s.scale < __int_as_float(0x7f800000));
+    s.scale = __fdiv_rn(top, BITS == 8 ? 127.f : 7.f);
+    const float inf = __int_as_float(0x7f800000);
+    const bool none = !(s.scale > 0.f && s.scale < inf);
     s.inv = none ? 0.f : __frcp_rn(s.scale);
-    s.half = 0.5f * s.scale;
+    s.half = none ? inf : s.scale < 7.888609e-31f ? 0.f : 0.5f * s.scale;
     return s;
 }
 
-// Codes of E values: round-half-even(x / scale), exactly as the quotient of real
-// numbers rounds.  x * inv is within 2^-22 of the quotient, so its rounding k is
-// off by one at most, and only next to a border between two codes.  The
-// remainder r = x - k scale is a multiple of the smaller of the two numbers'
-// last places and at most about scale / 2, so the fused multiply-add gives it
-// exactly: |r| < scale / 2 proves k, anything else (rare) is put right there.
-// 1.5 * 2^23 is added so that the sum's last bits are k itself.
-// Scales below 2^-100 (where half a step or 1 / scale leaves fp32's range) divide in fp64,
-// whose quotient of two fp32 numbers cannot round onto a border it is not on:
-// the two are 2^-33 apart at least, relative to the quotient.
-template <int BITS, int E>
-__device__ __forceinline__ void sq_codes(const float (&v)[E], const SqScale& s, uint32_t (&k)[E]) {
+// round-half-even(x / scale) in fp64, whose quotient of two fp32 numbers cannot
+// round onto a border between codes that it is not on: the two are 2^-33 apart at
+// least, relative to the quotient.
+template <int BITS>
+__device__ __noinline__ uint32_t sq_code_slow(float x, float scale) {
+    const double L = BITS == 8 ? 127.0 : 7.0;
+    return (uint32_t)(int)fmin(fmax(rint((double)x / (double)scale), -L), L);
+}
+
+// Codes of E values, packed as the store holds them: round-half-even(x / scale),
+// exactly as the quotient of real numbers rounds.  x * inv is within 2^-22 of
+// the quotient (relative), so its rounding k is off by one at most, and only next
+// to a border between two codes.  The remainder r = x - k scale is a multiple
+// of the smaller of the two numbers' last places and at most about scale / 2,
+// so the fused multiply-add gives it exactly: |r| < scale / 2 proves k; beyond it k
+// is one off, and on it the even neighbour is the code (both rare: one in
+// some 10^5 values).  1.5 * 2^23 is added so that the sum's last bits are k itself.
+template <typename T, int BITS, int E>
+__device__ __forceinline__ void sq_codes(const SqRaw<T, E>& x, const SqScale& s, uint32_t (&q)[(E * BITS + 31) / 32]) {
     constexpr float kMagic = 12582912.f;
-    if (s.inv == 0.f) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) k[e] = 0;
-        return;
-    }
-    if (s.scale < 7.888609e-31f) {
-        const double L = BITS == 8 ? 127.0 : 7.0;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            k[e] = (uint32_t)(int)fmin(fmax(rint((double)v[e] / (double)s.scale), -L), L);
-        return;
-    }
+    uint32_t k[E];
     float far = 0.f;
+    if constexpr (E == 1) {
+        const float v = x.get(0);
+        const float t = __fmaf_rn(v, s.inv, kMagic);
+        k[0] = __float_as_uint(t);
+        far = fabsf(__fmaf_rn(kMagic - t, s.scale, v));
+    } else {
+        const float2 inv = make_float2(s.inv, s.inv), sc = make_float2(-s.scale, -s.scale);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float t = __fmaf_rn(v[e], s.inv, kMagic);
-        k[e] = __float_as_uint(t);
-        far = fmaxf(far, fabsf(__fmaf_rn(-(t - kMagic), s.scale, v[e])));
+        for (int e = 0; e < E; e += 2) {
+            const float2 v = make_float2(x.get(e), x.get(e + 1));
+            const float2 t = sq_fma2(v, inv, make_float2(kMagic, kMagic));
+            k[e] = __float_as_uint(t.x);
+            k[e + 1] = __float_as_uint(t.y);
+            const float2 r = sq_fma2(sq_add2(t, make_float2(-kMagic, -kMagic)), sc, v);
+            far = fmaxf(far, fmaxf(fabsf(r.x), fabsf(r.y)));
+        }
     }
     if (far >= s.half) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float t = __uint_as_float(k[e]) - kMagic;
-            const float r = __fmaf_rn(-t, s.scale, v[e]);
-            const int i = (int)t;
-            k[e] = (uint32_t)(r > s.half || (r == s.half && (i & 1))      ? i + 1
-                              : r < -s.half || (r == -s.half && (i & 1)) ? i - 1
-                                                                         : i);
+            const float v = x.get(e), t = __uint_as_float(k[e]) - kMagic, r = __fmaf_rn(-t, s.scale, v);
+            const int i = (int)t, odd = i & 1;
+            if (s.half == 0.f) k[e] = sq_code_slow<BITS>(v, s.scale);
+            else k[e] = (uint32_t)(i + (r > s.half || (r == s.half && odd)) - (r < -s.half || (r == -s.half && odd)));
+        }
+    }
+    if constexpr (BITS == 8 && E % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i)
+            q[i] = __byte_perm(__byte_perm(k[4 * i], k[4 * i + 1], 0x0040),
+                               __byte_perm(k[4 * i + 2], k[4 * i + 3], 0x0040), 0x5410);
+    } else {
+        q[0] = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[0] |= (k[e] & ((1u << BITS) - 1u)) << (BITS * e);
+    }
+    // infinities and NaN reach the sums above: their groups' codes are 0 by choice
+#pragma unroll
+    for (int i = 0; i < (E * BITS + 31) / 32; ++i) q[i] = s.inv == 0.f ? 0u : q[i];
+}
+
+// stores the codes of values e0 .. e0 + E - 1 of a group of `width` values (e0 <
+// width) at cr (the group's first byte); values past the group's end are 0, so
+// the last odd value's byte has an empty high half
+template <typename T, int BITS, bool VEC, int E>
+__device__ __forceinline__ void sq_store(uint8_t* cr, int e0, int width, const SqRaw<T, E>& x, const SqScale& s) {
+    uint32_t q[(E * BITS + 31) / 32];
+    sq_codes<T, BITS, E>(x, s, q);
+    constexpr int W = E * BITS / 8;              // bytes of a chunk
+    uint8_t* to = cr + e0 * BITS / 8;
+    if constexpr (W == 8) *reinterpret_cast<uint2*>(to) = make_uint2(q[0], q[1]);
+    else if constexpr (W == 4) *reinterpret_cast<uint32_t*>(to) = q[0];
+    else if constexpr (W == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)q[0];
+    else to[0] = (uint8_t)q[0];
+}
+
+// W bytes of codes
+template <int W>
+__device__ __forceinline__ void sq_load_codes(const uint8_t* __restrict__ cr, uint32_t (&q)[(W + 3) / 4]) {
+    if constexpr (W == 8) {
+        const uint2 v = *reinterpret_cast<const uint2*>(cr);
+        q[0] = v.x;
+        q[1] = v.y;
+    } else if constexpr (W == 4) q[0] = *reinterpret_cast<const uint32_t*>(cr);
+    else if constexpr (W == 2) q[0] = *reinterpret_cast<const uint16_t*>(cr);
+    else q[0] = cr[0];
+}
+
+// the values of E codes.  A code c is put into the last bits of 2^23 (as c + 128,
+// or c + 8), and 2^23 + 128 (+ 8) taken away: whole numbers, exact in fp32.
+template <int BITS, int E>
+__device__ __forceinline__ void sq_values(const uint32_t (&q)[(E * BITS + 31) / 32], float scale, float (&v)[E]) {
+    constexpr uint32_t kBase = 0x4b000000u;
+    constexpr float kZero = BITS == 8 ? 8388736.f : 8388616.f;
+    const uint32_t lo = (q[0] & 0x0f0f0f0fu) ^ 0x08080808u, hi = ((q[0] >> 4) & 0x0f0f0f0fu) ^ 0x08080808u;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        v[e] = __uint_as_float(BITS == 8 ? __byte_perm(q[e >> 2] ^ 0x80808080u, kBase, 0x7440 | (e & 3))
+                                         : __byte_perm(e & 1 ? hi : lo, kBase, 0x7440 | (e >> 1)));
+    if constexpr (E == 1) v[0] = (v[0] - kZero) * scale;
+    else {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            const float2 r = sq_mul2(sq_add2(make_float2(v[e], v[e + 1]), make_float2(-kZero, -kZero)),
+                                     make_float2(scale, scale));
+            v[e] = r.x;
+            v[e + 1] = r.y;
         }
     }
 }
 
-// stores the codes of values e0 .. e0 + E - 1 of a group of `width` values at
-// cr (the group's first byte)
-template <int BITS, bool VEC, int E>
-__device__ __forceinline__ void sq_store(uint8_t* cr, int e0, int width, const float (&v)[E], const SqScale& s) {
-    uint32_t k[E];
-    sq_codes<BITS, E>(v, s, k);
-    constexpr int W = E * BITS / 8;              // bytes of a chunk
-    uint8_t by[W];
-#pragma unroll
-    for (int w = 0; w < W; ++w)
-        by[w] = BITS == 8 ? (uint8_t)k[w] : (uint8_t)((k[2 * w % E] & 15u) | ((k[(2 * w + 1) % E] & 15u) << 4));
-    const int b0 = e0 * BITS / 8;
-    if (VEC && e0 + E <= width) {
-        if constexpr (W == 8) *reinterpret_cast<uint2*>(cr + b0) = *reinterpret_cast<uint2*>(by);
-        else if constexpr (W == 4) *reinterpret_cast<uint32_t*>(cr + b0) = *reinterpret_cast<uint32_t*>(by);
-        else if constexpr (W == 2) *reinterpret_cast<uint16_t*>(cr + b0) = *reinterpret_cast<uint16_t*>(by);
-        else cr[b0] = by[0];
-    } else {
-        // values past the group's end are 0, so the last odd value's byte has an empty high half
-#pragma unroll
-        for (int w = 0; w < W; ++w)
-            if (e0 + w * 8 / BITS < width) cr[b0 + w] = by[w];
-    }
-}
-
-// W bytes of codes from byte b0 of a row of `bytes` bytes, 0 past its end
-template <bool VEC, int W>
-__device__ __forceinline__ void sq_load_codes(const uint8_t* __restrict__ cr, int b0, int bytes, uint8_t (&q)[W]) {
-    if (VEC && b0 + W <= bytes) {
-        if constexpr (W == 8) *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(cr + b0);
-        else if constexpr (W == 4) *reinterpret_cast<uint32_t*>(q) = *reinterpret_cast<const uint32_t*>(cr + b0);
-        else if constexpr (W == 2) *reinterpret_cast<uint16_t*>(q) = *reinterpret_cast<const uint16_t*>(cr + b0);
-        else q[0] = cr[b0];
-    } else {
-#pragma unroll
-        for (int w = 0; w < W; ++w) q[w] = b0 + w < bytes ? cr[b0 + w] : (uint8_t)0;
-    }
-}
-
-template <int BITS>
-__device__ __forceinline__ int sq_code(const uint8_t* q, int e) {
-    if (BITS == 8) return (int)(int8_t)q[e];
-    return (int)((int8_t)(uint8_t)(q[e >> 1] << (e & 1 ? 0 : 4)) >> 4);
-}
-
+// values e0 .. e0 + E - 1 of a row of d values; `once`: the caches need not keep them
 template <typename T, bool VEC, int E>
-__device__ __forceinline__ void sq_store_values(T* out, int e0, int d, const float (&v)[E]) {
-    T t[E];
+__device__ __forceinline__ void sq_store_values(T* out, int e0, int d, const float (&v)[E], bool once) {
+    if constexpr (VEC && sizeof(T) == 2) {
+        uint32_t w[E / 2];
 #pragma unroll
-    for (int e = 0; e < E; ++e) sq_round(v[e], t[e]);
-    if (VEC && e0 + E <= d) {
-        uint4 raw;
-        memcpy(&raw, t, 16);
-        *reinterpret_cast<uint4*>(out + e0) = raw;
+        for (int i = 0; i < E / 2; ++i) {
+            T t[2];
+            sq_round(v[2 * i], t[0]);
+            sq_round(v[2 * i + 1], t[1]);
+            memcpy(&w[i], t, 4);
+        }
+        const uint4 o = make_uint4(w[0], w[1], w[2], w[3]);
+        if (once) __stcs(reinterpret_cast<uint4*>(out + e0), o);
+        else *reinterpret_cast<uint4*>(out + e0) = o;
+    } else if constexpr (VEC) {
+        const float4 o = make_float4(v[0], v[1], v[2], v[3]);
+        if (once) __stcs(reinterpret_cast<float4*>(out + e0), o);
+        else *reinterpret_cast<float4*>(out + e0) = o;
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            if (e0 + e < d) out[e0 + e] = t[e];
+            if (e0 + e < d) sq_round(v[e], out[e0 + e]);
     }
 }
 
