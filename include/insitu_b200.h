@@ -327,7 +327,7 @@ int ivf_pq_encode(const void* d_x, int x_is_u8, long long n, int d, const int* d
  *   scale = fp32(max |x| over the group / L)
  *   code  = x / scale rounded to the nearest whole number, ties to even, in
  *           [-L, L]; 0 where the scale is 0
- *   value = code * scale, rounded once to the type it is read in
+ *   value = code * scale in fp32, rounded to the type it is read in
  * A group with a NaN or an infinity has that as its scale and reads as NaN.
  * No operator here has a gradient.
  *
@@ -351,7 +351,7 @@ int ivf_pq_encode(const void* d_x, int x_is_u8, long long n, int d, const int* d
 #define IVF_SQ_MAX_K 131071
 /*
  * Row i of d_x [n, d] (x_type, rows ldx values apart) is quantised into slot
- * d_slots[i] (NULL: slot i, then n <= capacity).  A row whose slot is outside
+ * d_slots[i] (NULL: slot i, then n <= capacity; capacity < 2^31).  A row whose slot is outside
  * [0, capacity) is left out; of rows with one slot the last stays; slots that no row names
  * are left as they were.  d_claim int32 [capacity] is scratch of any contents,
  * needed for more than IVF_SQ_SCAN_ROWS rows with slots (else it may be NULL).  n < 2^31.
@@ -380,12 +380,13 @@ int ivf_sq_matmul(const int8_t* d_a, long long lda, const float* d_a_scale, long
  * (x_type, rows ldx values apart) is quantised as ivf_sq_write does (bits 8,
  * group 0), then multiplied as by ivf_sq_matmul, with equal results.
  * d_scales dense [n].  d_work: scratch of ivf_sq_scores_work(m, d) bytes,
- * 16-byte aligned.
+ * 16-byte aligned (may be NULL where that is 0).
  */
 int ivf_sq_scores(const void* d_x, int x_type, long long ldx, long long m, const int8_t* d_codes, long long ldc,
                   const float* d_scales, long long n, int d, const float* d_bias, void* d_out, int out_type,
                   long long ldo, void* d_work, size_t work_bytes, void* stream);
-/* bytes of d_work that ivf_sq_scores needs (0 for sizes that it refuses) */
+/* bytes of d_work that ivf_sq_scores needs: 0 for a few tokens (and for sizes
+ * that it refuses) */
 size_t ivf_sq_scores_work(long long m, int d);
 
 /* ======================================================================

@@ -1558,7 +1558,7 @@ int ivf_sq_matmul(const int8_t* d_a, long long lda, const float* d_a_scale, long
 }
 
 size_t ivf_sq_scores_work(long long m, int d) {
-    if (m < 0 || m >= 2147483647ll || d < 1 || d > IVF_SQ_MAX_K) return 0;
+    if (m <= 0 || m >= 2147483647ll || d < 1 || d > IVF_SQ_MAX_K || sq_scores_fused(m, d)) return 0;
     return (size_t)m * (size_t)(sq_work_ld(d) + 4) + 16;
 }
 
@@ -1569,7 +1569,8 @@ int ivf_sq_scores(const void* d_x, int x_type, long long ldx, long long m, const
         need(d >= 1 && d <= IVF_SQ_MAX_K, "need 1 <= d <= IVF_SQ_MAX_K");
         sq_check_rows(d_x, x_type, m, d, ldx, "x");
         SqMatmul p = sq_check_product(d_codes, ldc, d_scales, m, n, d, d_bias, d_out, out_type, ldo);
-        need(work_bytes >= ivf_sq_scores_work(m, d) && d_work, "d_work is smaller than ivf_sq_scores_work(m, d)");
+        const size_t work = ivf_sq_scores_work(m, d);
+        need(work == 0 || (d_work && work_bytes >= work), "d_work is smaller than ivf_sq_scores_work(m, d)");
         need(reinterpret_cast<uintptr_t>(d_work) % 16 == 0, "d_work must be 16-byte aligned");
         if (m == 0 || n == 0) return;
         SqWrite w{};
@@ -1582,11 +1583,7 @@ int ivf_sq_scores(const void* d_x, int x_type, long long ldx, long long m, const
         w.scales = reinterpret_cast<float*>(w.codes + (size_t)m * w.ldc);
         w.lds = 1;
         w.capacity = (uint32_t)m;
-        ck(sq_write(w, x_type, 8, static_cast<cudaStream_t>(stream)), "sq_scores (quantise)");
-        p.a = reinterpret_cast<const int8_t*>(w.codes);
-        p.a_scale = w.scales;
-        p.lda = w.ldc;
-        ck(sq_matmul(p, out_type, static_cast<cudaStream_t>(stream)), "sq_scores (product)");
+        ck(sq_scores(w, x_type, p, out_type, static_cast<cudaStream_t>(stream)), "sq_scores");
     });
 }
 

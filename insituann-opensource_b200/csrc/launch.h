@@ -267,5 +267,10 @@ struct SqMatmul {
     int64_t ldo;
 };
 cudaError_t sq_matmul(const SqMatmul& p, int out_type, cudaStream_t st);
+// the product of the floating rows of w (x_type), quantised one scale a row
+// into w's codes and scales (or by the product itself); p without its tokens but for m
+cudaError_t sq_scores(const SqWrite& w, int x_type, SqMatmul p, int out_type, cudaStream_t st);
+// whether the product of m tokens quantises them itself (w's codes and scales are not used)
+bool sq_scores_fused(int64_t m, int k);
 
 }  // namespace isb

@@ -7,7 +7,7 @@
 //     scale = fp32(max |x| / L)
 //     code  = the whole number nearest to x / scale (ties to even), in [-L, L];
 //             0 where the scale is 0
-//     value = code * scale, rounded once to the type it is read in.
+//     value = code * scale in fp32, rounded to the type it is read in.
 // The scale is kept in fp32: 4 bytes a group, and an error of 2^-24 next to the
 // half step (2^-8 of the group's largest value at 8 bits) that the code costs.
 // A group with a NaN or an infinity keeps that NaN or infinity as its scale

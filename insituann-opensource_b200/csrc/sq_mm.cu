@@ -4,6 +4,8 @@
 // bits (k < 2^17); the scaling and the bias are fp32 and each output is
 // rounded once more, to its type.
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "launch.h"
 #include "sq.cuh"
@@ -18,112 +20,524 @@ __device__ __forceinline__ void mm_emit(T* out, int acc, float sa, float sb, flo
     sq_round(__fmaf_rn((float)acc * sa, sb, bias), *out);
 }
 
-// ---- tiles on the CUDA cores: any alignment --------------------------------
-// 64 x 64 outputs per block of 256 threads, 4 x 4 each by __dp4a; 64 bytes of k
-// per step through shared memory, stored by words of 4 k with the rows beside
-// each other (row index fastest), so that the threads of a warp read
-// neighbouring words.
-constexpr int kTile = 64, kStep = 64;
-
-__device__ __forceinline__ uint32_t mm_word(const int8_t* row, int t, int k, bool fast) {
-    if (fast && t + 4 <= k) return *reinterpret_cast<const uint32_t*>(row + t);
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (t + i < k) w |= (uint32_t)(uint8_t)row[t + i] << (8 * i);
-    return w;
+int sm_count() {
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return sms;
 }
 
+bool rows_aligned(const void* p, int64_t ld, int a) { return reinterpret_cast<uintptr_t>(p) % a == 0 && ld % a == 0; }
+
+// ---- up to 4 tokens: dot products on the CUDA cores ------------------------
+// With so few tokens every byte of b is used a handful of times, and the
+// product is the time to read b.  The tokens' codes lie in shared memory (each
+// block quantises them itself when they come as floating rows: one launch in
+// all).  A team of TEAM lanes takes R rows of b, 16 bytes a lane and row at a
+// time, so that several loads are in flight and each word of the tokens read
+// from shared memory serves R rows.  The teams' sums are joined by exchanging
+// halves: a lane ends up with its own outputs, V / TEAM of the V = MT * R.
+// 1 x 65536 x 128 with fp32 queries: 4.7 us (11.9 us as two launches, tiles for
+// the product); 1 x 1M x 128: 28.5 us, 4.8 TB/s.
+constexpr int kDotThreads = 256;
+constexpr int kDotTokens = 4;
+constexpr size_t kDotSmem = 72 * 1024;          // most shared memory for the tokens: three blocks an SM
+
+template <int MT, int R>
+constexpr int kDotCtas = MT * R <= 4 ? 3 : 2;   // blocks an SM that the registers of MT * R sums allow
+
+struct MmDot {
+    SqMatmul p;
+    const void* x;                              // floating tokens (null: p.a, p.a_scale)
+    int64_t ldx;
+    int x_type, out_type, x_vec;
+    int kp;                                     // bytes of a token's codes in shared memory
+};
+
+// 16 bytes of a row in flight: issue() starts the loads and has no branch, so
+// that several of them are under way at once; take() gives the bytes, with 0
+// past the row's end.  ALIGNED: rows are 16-byte aligned; else the two aligned
+// 16-byte pieces around the bytes are read and shifted.  A piece that is not
+// wholly inside the array [lo, hi) (at its ends only) is read by bytes.
+template <bool ALIGNED>
+struct MmBytes {
+    uint32_t v[ALIGNED ? 4 : 8];
+
+    // bytes [at, at + 16) of a row that ends at `end` (at >= end: none)
+    __device__ __forceinline__ void issue(uintptr_t at, uintptr_t end, uintptr_t lo, uintptr_t hi) {
+        if constexpr (ALIGNED) {
+            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+            if (at + 16 <= end) x = __ldg(reinterpret_cast<const uint4*>(at));
+            v[0] = x.x;
+            v[1] = x.y;
+            v[2] = x.z;
+            v[3] = x.w;
+        } else {
+            const uintptr_t w = at & ~uintptr_t(15);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                if (at < end && w + 16 * h < end && w + 16 * h >= lo && w + 16 * h + 16 <= hi)
+                    x = __ldg(reinterpret_cast<const uint4*>(w + 16 * h));
+                v[4 * h] = x.x;
+                v[4 * h + 1] = x.y;
+                v[4 * h + 2] = x.z;
+                v[4 * h + 3] = x.w;
+            }
+        }
+    }
+    __device__ __forceinline__ uint4 take(uintptr_t at, uintptr_t end, uintptr_t lo, uintptr_t hi) {
+        if constexpr (ALIGNED) {
+            if (at < end && at + 16 > end) {                     // the last bytes of a row
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = edge(at + 4 * i, at, end);
+            }
+            return make_uint4(v[0], v[1], v[2], v[3]);
+        } else {
+            const uintptr_t w = at & ~uintptr_t(15);
+            if (at < end && (w < lo || w + 32 > hi)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (w + (i & 4) * 4 < lo || w + (i & 4) * 4 + 16 > hi) v[i] = edge(w + 4 * i, lo, hi);
+            }
+            const uint4 x = shifted(at);
+            uint32_t o[4] = {x.x, x.y, x.z, x.w};
+            if (at + 16 > end) {                                 // clear what follows the row
+                const int left = at < end ? (int)(end - at) : 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int n = left - 4 * i;
+                    o[i] = n >= 4 ? o[i] : n <= 0 ? 0u : o[i] & ((1u << (8 * n)) - 1u);
+                }
+            }
+            return make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+    // the same where [at - 15, at + 32) is known to be inside the array and [at, at + 16) inside the row
+    __device__ __forceinline__ void issue_inside(uintptr_t at) {
+        const uint4* w = reinterpret_cast<const uint4*>(at & ~uintptr_t(15));
+        const uint4 x = __ldg(w), y = __ldg(w + 1);
+        v[0] = x.x;
+        v[1] = x.y;
+        v[2] = x.z;
+        v[3] = x.w;
+        v[4] = y.x;
+        v[5] = y.y;
+        v[6] = y.z;
+        v[7] = y.w;
+    }
+    // the 16 bytes from at & 15 on: by two words, by one, by bits
+    __device__ __forceinline__ uint4 shifted(uintptr_t at) {
+        const bool two = (at & 8) != 0, one = (at & 4) != 0;
+#pragma unroll
+        for (int i = 0; i < 6; ++i) v[i] = two ? v[i + 2] : v[i];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) v[i] = one ? v[i + 1] : v[i];
+        const uint32_t sh = (uint32_t)(at & 3) * 8;
+        return make_uint4(__funnelshift_r(v[0], v[1], sh), __funnelshift_r(v[1], v[2], sh),
+                          __funnelshift_r(v[2], v[3], sh), __funnelshift_r(v[3], v[4], sh));
+    }
+    // the word at w, 0 where its bytes are outside [lo, hi)
+    static __device__ __forceinline__ uint32_t edge(uintptr_t w, uintptr_t lo, uintptr_t hi) {
+        uint32_t x = 0;
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i)
+            if (w + i >= lo && w + i < hi) x |= (uint32_t)*reinterpret_cast<const uint8_t*>(w + i) << (8 * i);
+        return x;
+    }
+};
+
+// quantises one floating row of k values into shared memory (one scale), by the whole block
+template <typename T, bool VEC>
+__device__ __forceinline__ void dot_quantise(const T* x, int k, uint8_t* codes, float* scale, uint32_t* s_top) {
+    constexpr int E = sq_chunk<T, 8, VEC>();
+    uint32_t top = 0;
+    for (int e0 = threadIdx.x * E; e0 < k; e0 += kDotThreads * E) sq_load<T, VEC, E>(x, e0, k).top(top);
+    top = __reduce_max_sync(0xffffffffu, __float_as_uint(sq_top<T>(top)));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = 0;
+#pragma unroll
+    for (int w = 0; w < kDotThreads / 32; ++w) top = max(top, s_top[w]);
+    const SqScale s = sq_scale<8>(__uint_as_float(top));
+    for (int e0 = threadIdx.x * E; e0 < k; e0 += kDotThreads * E)
+        sq_store<T, 8, VEC, E>(codes, e0, k, sq_load<T, VEC, E>(x, e0, k), s);
+    if (threadIdx.x == 0) *scale = s.scale;
+}
 template <typename T>
-__global__ void __launch_bounds__(256) mm_tile_kernel(SqMatmul p, int fast_a, int fast_b, int tiles_n) {
-    __shared__ uint32_t sa[kStep / 4][kTile + 1], sb[kStep / 4][kTile + 1];
-    const int64_t i0 = (int64_t)(blockIdx.x / tiles_n) * kTile, j0 = (int64_t)(blockIdx.x % tiles_n) * kTile;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    for (int t0 = 0; t0 < p.k; t0 += kStep) {
+__device__ __forceinline__ void dot_quantise(const MmDot& q, int i, uint8_t* codes, float* scale, uint32_t* s_top) {
+    const T* x = static_cast<const T*>(q.x) + i * q.ldx;
+    if (q.x_vec) dot_quantise<T, true>(x, q.p.k, codes, scale, s_top);
+    else dot_quantise<T, false>(x, q.p.k, codes, scale, s_top);
+}
+
+// sums acc[0 .. N) over the 2 O lanes that differ in the bits below 2 O; the lane's
+// share, N / (2 O) values (or one, held by several lanes), is left in
+// acc[0 ..): values from the returned index on
+template <int N, int O, int V>
+__device__ __forceinline__ int dot_join(int (&acc)[V], int tl) {
+    if constexpr (O == 0) return 0;
+    else if constexpr (N > 1) {
+        const bool up = (tl & O) != 0;
 #pragma unroll
-        for (int u = 0; u < kTile * kStep / 4 / 256; ++u) {
-            const int w = threadIdx.x + 256 * u, r = w / (kStep / 4), c = w % (kStep / 4);
-            sa[c][r] = i0 + r < p.m ? mm_word(p.a + (i0 + r) * p.lda, t0 + 4 * c, p.k, fast_a) : 0u;
-            sb[c][r] = j0 + r < p.n ? mm_word(p.b + (j0 + r) * p.ldb, t0 + 4 * c, p.k, fast_b) : 0u;
+        for (int q = 0; q < N / 2; ++q) {
+            const int give = up ? acc[q] : acc[q + N / 2], keep = up ? acc[q + N / 2] : acc[q];
+            acc[q] = keep + __shfl_xor_sync(0xffffffffu, give, O);
         }
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < kStep / 4; ++c) {
-            int av[4], bv[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) av[i] = (int)sa[c][ty + 16 * i];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) bv[j] = (int)sb[c][tx + 16 * j];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(av[i], bv[j], acc[i][j]);
-        }
-        __syncthreads();
+        return (up ? N / 2 : 0) + dot_join<N / 2, O / 2, V>(acc, tl);
+    } else {
+        acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], O);
+        return dot_join<1, O / 2, V>(acc, tl);
     }
-    T* out = static_cast<T*>(p.out);
+}
+
+template <int MT, int TEAM, int R, bool ALIGNED>
+__global__ void __launch_bounds__(kDotThreads, kDotCtas<MT, R>) mm_dot_kernel(MmDot q) {
+    constexpr int V = MT * R, NV = V / TEAM > 0 ? V / TEAM : 1;
+    constexpr int TEAMS = kDotThreads / TEAM;
+    extern __shared__ __align__(16) uint8_t s_a[];               // [MT][kp]
+    __shared__ float s_scale[MT];
+    __shared__ uint32_t s_top[kDotThreads / 32];
+    const SqMatmul& p = q.p;
+    const int m = (int)p.m;
+    const int tl = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+
+    for (int i = 0; i < MT; ++i) {
+        uint8_t* row = s_a + (size_t)i * q.kp;
+        if (i >= m) {
+            for (int t = threadIdx.x; t < q.kp / 16; t += kDotThreads)
+                reinterpret_cast<uint4*>(row)[t] = make_uint4(0u, 0u, 0u, 0u);
+            if (threadIdx.x == 0) s_scale[i] = 0.f;
+        } else if (q.x) {
+            for (int t = p.k + threadIdx.x; t < q.kp; t += kDotThreads) row[t] = 0;
+            if (q.x_type == kSqF32) dot_quantise<float>(q, i, row, s_scale + i, s_top);
+            else if (q.x_type == kSqF16) dot_quantise<__half>(q, i, row, s_scale + i, s_top);
+            else dot_quantise<__nv_bfloat16>(q, i, row, s_scale + i, s_top);
+        } else {
+            const uintptr_t lo = reinterpret_cast<uintptr_t>(p.a), hi = lo + (m - 1) * p.lda + p.k;
+            const uintptr_t a = lo + i * p.lda;
+            for (int t = threadIdx.x; t < q.kp / 16; t += kDotThreads) {
+                MmBytes<false> w;
+                w.issue(a + 16 * t, a + p.k, lo, hi);
+                reinterpret_cast<uint4*>(row)[t] = w.take(a + 16 * t, a + p.k, lo, hi);
+            }
+            if (threadIdx.x == 0) s_scale[i] = p.a_scale[i];
+        }
+    }
+    __syncthreads();
+
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p.b), hi = lo + (p.n - 1) * p.ldb + p.k;
+    const int64_t step = (int64_t)gridDim.x * (TEAMS * R);
+    // the loop bound is the same for a warp's teams: all lanes take part in every exchange
+    for (int64_t j0 = (int64_t)blockIdx.x * (TEAMS * R); j0 < p.n; j0 += step) {
+        const int64_t j = j0 + team * R;
+        uintptr_t b[R], end[R];                                  // a row past the last one is empty
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t col = j0 + tx + 16 * j;
-        if (col >= p.n) continue;
-        const float s = p.b_scale[col], bias = p.bias ? p.bias[col] : 0.f;
+        for (int r = 0; r < R; ++r) {
+            b[r] = lo + (j + r < p.n ? j + r : 0) * p.ldb;
+            end[r] = b[r] + (j + r < p.n ? p.k : 0);
+        }
+        int acc[V];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t row = i0 + ty + 16 * i;
-            if (row < p.m) mm_emit(out + row * p.ldo + col, acc[i][j], p.a_scale[row], s, bias);
+        for (int v = 0; v < V; ++v) acc[v] = 0;
+#pragma unroll R <= 2 ? 8 / R : 2
+        for (int t = tl * 16; t < q.kp; t += TEAM * 16) {
+            MmBytes<ALIGNED> raw[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) raw[r].issue(b[r] + t, end[r], lo, hi);
+            uint4 w[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) w[r] = raw[r].take(b[r] + t, end[r], lo, hi);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const uint4 a = *reinterpret_cast<const uint4*>(s_a + (size_t)i * q.kp + t);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    int s = acc[i * R + r];
+                    s = __dp4a((int)a.x, (int)w[r].x, s);
+                    s = __dp4a((int)a.y, (int)w[r].y, s);
+                    s = __dp4a((int)a.z, (int)w[r].z, s);
+                    acc[i * R + r] = __dp4a((int)a.w, (int)w[r].w, s);
+                }
+            }
+        }
+        const int v0 = dot_join<V, TEAM / 2, V>(acc, tl);
+        if (V < TEAM && (tl & (TEAM / V - 1)) != 0) continue;    // one of the lanes that hold a value stores it
+#pragma unroll
+        for (int e = 0; e < NV; ++e) {
+            const int i = (v0 + e) / R;
+            const int64_t col = j + (v0 + e) % R;
+            if (i >= m || col >= p.n) continue;
+            const float sb = p.b_scale[col], bias = p.bias ? p.bias[col] : 0.f;
+            const int64_t at = i * p.ldo + col;
+            if (q.out_type == kSqF32) mm_emit(static_cast<float*>(p.out) + at, acc[e], s_scale[i], sb, bias);
+            else if (q.out_type == kSqF16) mm_emit(static_cast<__half*>(p.out) + at, acc[e], s_scale[i], sb, bias);
+            else mm_emit(static_cast<__nv_bfloat16*>(p.out) + at, acc[e], s_scale[i], sb, bias);
         }
     }
 }
 
-// ---- tiles on the tensor cores: 16-byte aligned rows ------------------------
+template <int MT, int TEAM, int R, bool ALIGNED>
+cudaError_t go_dot(const MmDot& q, cudaStream_t st) {
+    const size_t smem = (size_t)MT * q.kp;
+    if (smem > 40 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(mm_dot_kernel<MT, TEAM, R, ALIGNED>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kDotSmem);
+        if (e) return e;
+    }
+    const int64_t per = kDotThreads / TEAM * R;
+    const int grid = (int)std::min<int64_t>((q.p.n + per - 1) / per, (int64_t)sm_count() * kDotCtas<MT, R>);
+    note_launch();
+    mm_dot_kernel<MT, TEAM, R, ALIGNED><<<grid, kDotThreads, smem, st>>>(q);
+    return cudaGetLastError();
+}
+
+// Rows of up to 128 bytes: 8 lanes a row, so that a warp reads 4 rows at once.
+// Longer ones take the warp; a single token takes fewer rows a warp where there
+// are few rows, so that all SMs have warps (1 x 4096 x 4096: 9.3 us with 4 rows, 7.3 us with 2).
+template <int MT, bool ALIGNED>
+cudaError_t by_team(const MmDot& q, cudaStream_t st) {
+    if (q.kp <= 128) return go_dot<MT, 8, MT == 1 ? 8 : 4, ALIGNED>(q, st);
+    if constexpr (MT == 1) {
+        if (q.p.n < 4096) return go_dot<MT, 32, 1, ALIGNED>(q, st);
+        if (q.p.n < 10000) return go_dot<MT, 32, 2, ALIGNED>(q, st);
+    }
+    return go_dot<MT, 32, 4, ALIGNED>(q, st);
+}
+
+// bytes of a token's codes that a team's lanes read: whole steps of the team
+int dot_kp(int k) {
+    const int step = k <= 128 ? 128 : 512;
+    return (k + step - 1) / step * step;
+}
+
+bool dot_usable(const SqMatmul& p) {
+    const int mt = p.m == 1 ? 1 : kDotTokens;
+    return p.m <= kDotTokens && (size_t)mt * dot_kp(p.k) <= kDotSmem;
+}
+
+cudaError_t launch_dot(MmDot q, cudaStream_t st) {
+    q.kp = dot_kp(q.p.k);
+    const bool al = rows_aligned(q.p.b, q.p.ldb, 16);
+    if (q.p.m == 1) return al ? by_team<1, true>(q, st) : by_team<1, false>(q, st);
+    return al ? by_team<kDotTokens, true>(q, st) : by_team<kDotTokens, false>(q, st);
+}
+
+// ---- tiles on the tensor cores ---------------------------------------------
 // tcgen05.mma kind::i8, s8 x s8 summed exactly in s32 in tensor memory.  The
 // channels (rows of b) are the MMA's M, 128 a tile, and the tokens (rows of a)
 // its N, NT a tile, so that 1 to 256 tokens fit one tile without padding to
 // 128, and accumulator lane i is channel i: the 32 lanes of an epilogue warp
 // store 32 neighbouring outputs of one token with no exchange between them.
 //
-// A CTA takes tiles t = blockIdx.x, + gridDim.x, ...:
-//   warp 0      one lane issues the tensor copies, 128 bytes of k of the tile's
-//               rows of b and a per stage, 128-byte swizzled, through tensor
-//               maps over this GPU's memory (no multicast); rows and bytes past
-//               the ends read as zeros;
+// A unit of work is a tile, or, with `split` > 1, one of the `split` parts of a
+// tile's k; a CTA takes the units blockIdx.x, + gridDim.x, ... (one unit each when
+// k is split):
+//   warp 0      (TMA) one lane issues the tensor copies, 128 bytes of k of the
+//               tile's rows of b and a per stage, 128-byte swizzled, through
+//               tensor maps over this GPU's memory (no multicast); rows and
+//               bytes past the ends read as zeros;
+//   last warps  (not TMA: rows that are not 16-byte aligned) kLoad warps put 16
+//               bytes together from aligned words and store them where the
+//               tensor copy would;
 //   warp 1      allocates tensor memory; one lane issues the MMAs (32 bytes of
 //               k each) into one of two accumulators of NT columns;
 //   warps 2..   epilogue: scales, bias, rounding and stores, while the next
 //               tile's MMAs run.
-// Every wait is bounded; after a wait that gives up the CTA's remaining outputs are NaN.
+// The parts of a split tile are the CTAs of one cluster: each leaves its sums in
+// its shared memory and adds up, over the cluster, the columns that fall to
+// it (whole numbers: the order does not matter).
+// Every wait on a barrier in memory is bounded; after one that gives up the CTA's
+// remaining outputs are NaN.
 constexpr int kMmM = 128, kMmK = 128;
+constexpr int kMmMaxStages = 12;
 
-template <int NT>
+template <int NT, bool TMA>
 struct MmCfg {
     static constexpr int kStage = (kMmM + NT) * kMmK;
-    static constexpr int kFit = (227 * 1024 - 1024 - 4096) / kStage;
-    static constexpr int kStages = kFit < 12 ? kFit : 12;
-    static constexpr int kEpi = NT >= 64 ? 8 : 4;                 // epilogue warps
-    static constexpr int kThreads = 64 + 32 * kEpi;
+    static constexpr int kEpi = !TMA ? 4 : NT >= 256 ? 16 : NT >= 64 ? 8 : 4;   // epilogue warps
+    static constexpr int kLoad = TMA ? 0 : 16;                    // loading warps
+    static constexpr int kThreads = 64 + 32 * (kEpi + kLoad);
+    static constexpr int kCtas = TMA && NT <= 128 ? 2 : 1;        // resident per SM
     static constexpr int kCols = 2 * NT;                          // tensor-memory columns
     static constexpr int kHalf = NT / (kEpi / 4);                 // columns of an epilogue warp
     static constexpr int kChunk = kHalf < 32 ? kHalf : 32;
+    static constexpr int kStatic = kEpi * kChunk * 4 + 1024;   // static arrays and the system's 1 KB
+    static constexpr int kFit = (227 * 1024 / kCtas - 1024 - 1024 - kStatic) / kStage;
+    static constexpr int kStages = kFit < kMmMaxStages ? kFit : kMmMaxStages;
     static constexpr size_t kSmem = (size_t)kStage * kStages + 1024;
+    static_assert(kStages >= 2 && (size_t)kMmM * NT * 4 <= (size_t)kStage * kStages, "a split tile's sums fit the stages");
 };
 
 // tile t of tn channel tiles x tm token tiles: bands of 8 token tiles, so that
-// the CTAs at work share rows of both operands in L2
-__device__ __forceinline__ void mm_place(int64_t t, int tn, int tm, int& ct, int& tt) {
-    const int64_t per = (int64_t)8 * tn;
-    const int band = (int)(t / per);
-    const int w = min(8, tm - 8 * band);
-    const uint32_t r = (uint32_t)(t - band * per);               // below 8 * 2^24
-    ct = (int)(r / (uint32_t)w);
-    tt = 8 * band + (int)(r - (uint32_t)ct * (uint32_t)w);
+// the CTAs at work share rows of both operands in L2.  32-bit divisions: 64-bit
+// ones took a third of the epilogue's instructions at k = 128.
+__device__ __forceinline__ void mm_place(uint32_t t, uint32_t tn, uint32_t tm, int& ct, int& tt) {
+    const uint32_t per = 8 * tn, band = t / per, w = min(8u, tm - 8 * band), r = t - band * per;
+    ct = (int)(r / w);
+    tt = (int)(8 * band + r - (uint32_t)ct * w);
 }
 
-template <typename T, int NT>
-__global__ void __launch_bounds__(MmCfg<NT>::kThreads, 1)
-    mm_tc_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a, SqMatmul p,
-                 int tn, int tm) {
-    using C = MmCfg<NT>;
+// wait on an mbarrier phase, suspended, bounded by kTCWaitNs of wall time; false where it gave up
+__device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, const volatile int* fail) {
+    if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+    return mbar_wait_timed(bar, parity, fail);
+}
+
+// The copying and the MMA thread run once per 128 bytes of k, some 500 clocks of
+// the tensor core: their place in the ring of stages is counted, not divided out (a 64-bit
+// remainder a step cost a fifth of the rate).
+struct MmRing {
+    uint32_t s = 0, lap = 0;                    // stage, times round the ring
+    __device__ __forceinline__ void next(uint32_t stages) {
+        if (++s == stages) {
+            s = 0;
+            ++lap;
+        }
+    }
+};
+
+// waits until every phase of a ring's stages that was begun is over
+__device__ __forceinline__ void mm_drain(uint64_t* bars, MmRing r, uint32_t stages) {
+    for (uint32_t i = 0; i < stages; ++i) {
+        // stage i was last used in lap `lap` where i is before the ring's place, else in the lap before
+        if (i < r.s) mm_wait(bars + i, r.lap & 1, nullptr);
+        else if (r.lap > 0) mm_wait(bars + i, (r.lap - 1) & 1, nullptr);
+    }
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// the 32-bit word at shared-memory address `at` of CTA `rank` of the cluster
+__device__ __forceinline__ int cluster_load(uint32_t at, int rank) {
+    uint32_t remote;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+    return v;
+}
+
+// the 16 bytes there
+__device__ __forceinline__ int4 cluster_load4(uint32_t at, int rank) {
+    uint32_t remote;
+    int4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(remote)
+                 : "memory");
+    return v;
+}
+
+// one MMA: accumulator d, channels' descriptor b, tokens' descriptor a
+__device__ __forceinline__ void mm_issue(uint32_t d, uint64_t b, uint64_t a, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred pa;\n setp.ne.b32 pa, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, pa;\n}" ::"r"(d),
+        "l"(b), "l"(a), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+struct MmTc {
+    SqMatmul p;
+    int out_type;
+    uint32_t tn, tm;            // channel and token tiles, fewer than 2^31 in all
+    int split;                  // parts of k (the cluster's size)
+    int kb_part;                // 128-byte blocks of k per part
+    bool pair;                  // 2 neighbouring 16-bit outputs may be stored at once
+};
+
+// Outputs of an epilogue warp: 32 channels (one a lane, `nch` of them there) of
+// `cnt` tokens (at most N) from `o` on (the lane's channel), rows ldo values apart.
+//
+// With output-bound products (k near 128) the instructions of this loop decide.
+// Two tokens are scaled at once by packed fp32 pairs; sums of at most 2^22
+// (SMALL: k <= 256) become floats by adding 1.5 * 2^23 as bits, which is exact
+// and leaves the slow integer conversion out; and 16-bit outputs (PAIR: rows
+// 4-byte aligned) are exchanged with the neighbouring lane, so that each lane
+// stores 2 channels of one token.  Turning the block in shared memory for 16-byte stores was slower (fp32
+// scores of 256 x 1M: 283 against 222 us): its round trips wait longer than the stores saved.
+template <bool SMALL>
+__device__ __forceinline__ float2 mm_scaled(uint32_t v0, uint32_t v1, float2 sa, float sb, float bias) {
+    constexpr float kMagic = 12582912.f;
+    const float2 f = SMALL ? sq_add2(make_float2(__uint_as_float(0x4b400000u + v0), __uint_as_float(0x4b400000u + v1)),
+                                     make_float2(-kMagic, -kMagic))
+                           : make_float2((float)(int)v0, (float)(int)v1);
+    return sq_fma2(sq_mul2(f, sa), make_float2(sb, sb), make_float2(bias, bias));
+}
+
+__device__ __forceinline__ uint32_t mm_pack(float2 r, __half) {
+    const __half2 h = __floats2half2_rn(r.x, r.y);
+    uint32_t w;
+    memcpy(&w, &h, 4);
+    return w;
+}
+__device__ __forceinline__ uint32_t mm_pack(float2 r, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(r.x, r.y);
+    uint32_t w;
+    memcpy(&w, &h, 4);
+    return w;
+}
+
+template <typename T, int N, bool SMALL>
+__device__ __forceinline__ void mm_block(T* o, int64_t ldo, const uint32_t (&v)[N], const float* sc, int cnt, float sb,
+                                         float bias, int nch, int lane, bool pair) {
+    if constexpr (sizeof(T) == 2) {
+        if (pair && cnt == N && nch >= 32) {
+            const int odd = lane & 1;
+            o += odd ? ldo - 1 : 0;                              // an odd lane stores the second token
+#pragma unroll
+            for (int j = 0; j < N; j += 2) {
+                const uint32_t w = mm_pack(mm_scaled<SMALL>(v[j], v[j + 1], *reinterpret_cast<const float2*>(sc + j), sb,
+                                                            bias),
+                                           T{});
+                const uint32_t x = __shfl_xor_sync(0xffffffffu, w, 1);
+                const uint32_t y = __byte_perm(w, x, odd ? 0x3276 : 0x5410);
+                *reinterpret_cast<uint32_t*>(o) = y;
+                o += 2 * ldo;
+            }
+            return;
+        }
+    }
+    if (lane >= nch) return;
+    if (cnt == N) {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const float2 r = mm_scaled<SMALL>(v[j], v[j + 1], *reinterpret_cast<const float2*>(sc + j), sb, bias);
+            sq_round(r.x, o[0]);
+            sq_round(r.y, o[ldo]);
+            o += 2 * ldo;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (j < cnt) mm_emit(o, (int)v[j], sc[j], sb, bias);
+            o += ldo;
+        }
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void mm_block(const MmTc& q, int64_t at, const uint32_t (&v)[N], const float* sc, int cnt,
+                                         float sb, float bias, int nch, int lane) {
+    auto go = [&](auto* out) {
+        using T = std::remove_pointer_t<decltype(out)>;
+        if (q.p.k <= 256) mm_block<T, N, true>(out + at, q.p.ldo, v, sc, cnt, sb, bias, nch, lane, q.pair);
+        else mm_block<T, N, false>(out + at, q.p.ldo, v, sc, cnt, sb, bias, nch, lane, q.pair);
+    };
+    if (q.out_type == kSqF32) go(static_cast<float*>(q.p.out));
+    else if (q.out_type == kSqF16) go(static_cast<__half*>(q.p.out));
+    else go(static_cast<__nv_bfloat16*>(q.p.out));
+}
+
+template <int NT, bool TMA>
+__global__ void __launch_bounds__(MmCfg<NT, TMA>::kThreads, MmCfg<NT, TMA>::kCtas)
+    mm_tc_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
+                 const __grid_constant__ MmTc q) {
+    using C = MmCfg<NT, TMA>;
     extern __shared__ unsigned char sm_raw[];
     unsigned char* sm =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
@@ -134,10 +548,14 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, 1)
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
     __shared__ __align__(16) float s_scale[C::kEpi][C::kChunk];
+    const SqMatmul& p = q.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const volatile int* vfail = &s_fail;
-    const int64_t tiles = (int64_t)tn * tm;
-    const int kblocks = (p.k + kMmK - 1) / kMmK;
+    const int split = q.split, part = split > 1 ? (int)(blockIdx.x % split) : 0;
+    const uint32_t t0 = split > 1 ? blockIdx.x / split : blockIdx.x;
+    const uint32_t tiles = split > 1 ? t0 + 1 : q.tn * q.tm;              // one past this CTA's last
+    const int kb0 = part * q.kb_part;
+    const int kb1 = min(kb0 + q.kb_part, (p.k + kMmK - 1) / kMmK);
 
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
@@ -147,7 +565,7 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, 1)
     }
     if (tid == 0) {
         for (int s = 0; s < C::kStages; ++s) {
-            mbar_init(&bar_full[s], 1);
+            mbar_init(&bar_full[s], TMA ? 1 : 4);                // the copying lane, or the warps of a loading group
             mbar_init(&bar_empty[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -163,56 +581,51 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, 1)
     const uint32_t tmem = s_tmem;
 
     if (warp == 0) {
-        if (lane == 0) {
-            int64_t g = 0;                                       // stages filled so far
-            for (int64_t t = blockIdx.x; t < tiles && !*vfail; t += gridDim.x) {
+        if (TMA && lane == 0) {
+            MmRing r;
+            for (uint32_t t = t0; t < tiles && !*vfail; t += gridDim.x) {
                 int ct, tt;
-                mm_place(t, tn, tm, ct, tt);
-                for (int kb = 0; kb < kblocks; ++kb, ++g) {
-                    const int s = (int)(g % C::kStages);
-                    if (g >= C::kStages &&
-                        !mbar_wait_timed(&bar_empty[s], (uint32_t)((g / C::kStages - 1) & 1), vfail)) {
+                mm_place(t, q.tn, q.tm, ct, tt);
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (r.lap > 0 && !mm_wait(&bar_empty[r.s], (r.lap - 1) & 1, vfail)) {
                         s_fail = 1;
                         break;
                     }
-                    unsigned char* st = sm + (size_t)s * C::kStage;
-                    mbar_arrive_expect(&bar_full[s], C::kStage);
-                    tma_load_2d(st, &map_b, kb * kMmK, ct * kMmM, &bar_full[s]);
-                    tma_load_2d(st + kMmM * kMmK, &map_a, kb * kMmK, tt * NT, &bar_full[s]);
+                    unsigned char* st = sm + (size_t)r.s * C::kStage;
+                    mbar_arrive_expect(&bar_full[r.s], C::kStage);
+                    tma_load_2d(st, &map_b, kb * kMmK, ct * kMmM, &bar_full[r.s]);
+                    tma_load_2d(st + kMmM * kMmK, &map_a, kb * kMmK, tt * NT, &bar_full[r.s]);
+                    r.next(C::kStages);
                 }
             }
             // the copies in flight land before the CTA's shared memory is released
-            for (int64_t i = g > C::kStages ? g - C::kStages : 0; i < g; ++i)
-                mbar_wait_timed(&bar_full[i % C::kStages], (uint32_t)((i / C::kStages) & 1), nullptr);
+            mm_drain(bar_full, r, C::kStages);
         }
         __syncwarp();
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc = umma_idesc_s8(kMmM, NT);
-            int64_t g = 0, n = 0;                                // stages read, tiles done
-            for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
-                const int a = (int)(n & 1);
-                bool ok = n < 2 || mbar_wait_timed(&bar_ae[a], (uint32_t)((n / 2 - 1) & 1), vfail);
-                const uint32_t dacc = tmem + (uint32_t)(a * NT);
-                for (int kb = 0; ok && kb < kblocks; ++kb, ++g) {
-                    const int s = (int)(g % C::kStages);
-                    ok = mbar_wait_timed(&bar_full[s], (uint32_t)((g / C::kStages) & 1), vfail);
+            const uint64_t desc0 = umma_smem_desc_sw128(smem_u32(sm));
+            const int last = (p.k - (kb1 - 1) * kMmK + 31) / 32;          // MMAs of the last step of k (1 to 4 are needed)
+            MmRing r;
+            uint32_t n = 0;                                      // tiles done
+            for (uint32_t t = t0; t < tiles; t += gridDim.x, ++n) {
+                const uint32_t a = n & 1;
+                bool ok = n < 2 || mm_wait(&bar_ae[a], (n / 2 - 1) & 1, vfail);
+                const uint32_t dacc = tmem + a * NT;
+                for (int kb = kb0; ok && kb < kb1; ++kb) {
+                    ok = mm_wait(&bar_full[r.s], r.lap & 1, vfail);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t b_addr = smem_u32(sm + (size_t)s * C::kStage);
-                    const uint32_t a_addr = b_addr + kMmM * kMmK;
-                    const int steps = min(4, (p.k - kb * kMmK + 31) / 32);
-                    for (int kk = 0; kk < steps; ++kk) {
-                        const uint64_t bd = umma_smem_desc_sw128(b_addr + 32 * kk);
-                        const uint64_t ad = umma_smem_desc_sw128(a_addr + 32 * kk);
-                        const uint32_t acc = kb | kk ? 1u : 0u;
-                        asm volatile(
-                            "{\n .reg .pred pa;\n setp.ne.b32 pa, %4, 0;\n"
-                            " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, pa;\n}" ::"r"(dacc),
-                            "l"(bd), "l"(ad), "r"(idesc), "r"(acc)
-                            : "memory");
-                    }
-                    tc_commit(&bar_empty[s]);
+                    // descriptor addresses count 16 bytes; one MMA reads 32 bytes of k
+                    const uint64_t bd = desc0 + r.s * (C::kStage >> 4), ad = bd + (kMmM * kMmK >> 4);
+                    mm_issue(dacc, bd, ad, idesc, kb > kb0);
+                    const int steps = kb + 1 == kb1 ? last : 4;
+                    if (steps > 1) mm_issue(dacc, bd + 2, ad + 2, idesc, 1);
+                    if (steps > 2) mm_issue(dacc, bd + 4, ad + 4, idesc, 1);
+                    if (steps > 3) mm_issue(dacc, bd + 6, ad + 6, idesc, 1);
+                    tc_commit(&bar_empty[r.s]);
+                    r.next(C::kStages);
                 }
                 if (!ok) {
                     s_fail = 1;
@@ -221,34 +634,52 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, 1)
                 tc_commit(&bar_af[a]);
             }
             // the MMAs in flight are done before tensor memory and the stages are released
-            const int64_t last = n - 1;
-            if (n > 0) mbar_wait_timed(&bar_af[last & 1], (uint32_t)((last / 2) & 1), nullptr);
-            for (int64_t i = g > C::kStages ? g - C::kStages : 0; i < g; ++i)
-                mbar_wait_timed(&bar_empty[i % C::kStages], (uint32_t)((i / C::kStages) & 1), nullptr);
+            mm_drain(bar_empty, r, C::kStages);
         }
         __syncwarp();
-    } else {
-        const int ew = warp - 2, quarter = warp & 3, part = ew >> 2;
+    } else if (warp < 2 + C::kEpi) {
+        const int ew = warp - 2, quarter = warp & 3, side = ew >> 2;
         float* sc = s_scale[ew];
-        T* out = static_cast<T*>(p.out);
-        int64_t n = 0;
+        uint32_t n = 0;                                          // tiles done
         bool ok = true;
-        for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
-            int ct, tt;
-            mm_place(t, tn, tm, ct, tt);
-            const int a = (int)(n & 1);
-            const int64_t ch = (int64_t)ct * kMmM + quarter * 32 + lane;
-            const bool in = ch < p.n;
-            const float sb = in ? p.b_scale[ch] : 0.f;
-            const float bias = in && p.bias ? p.bias[ch] : 0.f;
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait_timed(&bar_af[a], (uint32_t)((n / 2) & 1), vfail));
+        // a tile's place, channel scale and bias are found a tile ahead
+        int ct_next = 0, tt_next = 0;
+        float sb_next = 0.f, bias_next = 0.f;
+        auto fetch = [&](uint32_t t) {
+            mm_place(t, q.tn, q.tm, ct_next, tt_next);
+            const int64_t ch = (int64_t)ct_next * kMmM + quarter * 32 + lane;
+            if (ch < p.n) {
+                sb_next = p.b_scale[ch];
+                bias_next = p.bias ? p.bias[ch] : 0.f;
+            }
+        };
+        if (t0 < tiles) fetch(t0);
+        for (uint32_t t = t0; t < tiles; t += gridDim.x, ++n) {
+            const int a = (int)(n & 1), tt = tt_next;
+            const int64_t ch = (int64_t)ct_next * kMmM + quarter * 32 + lane;
+            const float sb = sb_next, bias = bias_next;
+            if (t + gridDim.x < tiles) fetch(t + gridDim.x);
+            if (ok) ok = __all_sync(0xffffffffu, mm_wait(&bar_af[a], (n / 2) & 1, vfail));
             if (!ok && lane == 0) s_fail = 1;
             tc_fence_after();
+            if (split > 1) {
+                // this part's sums to shared memory (the stages are read: the accumulator is done), [column][channel]
+                int* x = reinterpret_cast<int*>(sm) + (size_t)side * C::kHalf * kMmM + quarter * 32 + lane;
+                for (int c = 0; c < C::kHalf; c += C::kChunk) {
+                    uint32_t v[C::kChunk];
+                    const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(side * C::kHalf + c);
+                    if constexpr (C::kChunk == 32) tmem_ld32(ta, v);
+                    else tmem_ld16(ta, v);
+#pragma unroll
+                    for (int j = 0; j < C::kChunk; ++j) x[(size_t)(c + j) * kMmM] = (int)v[j];
+                }
+                break;
+            }
             for (int c = 0; c < C::kHalf; c += C::kChunk) {
-                const int64_t tok = (int64_t)tt * NT + part * C::kHalf + c;
+                const int64_t tok = (int64_t)tt * NT + side * C::kHalf + c;
                 uint32_t v[C::kChunk];
                 if (ok) {
-                    const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(a * NT + part * C::kHalf + c);
+                    const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(a * NT + side * C::kHalf + c);
                     if constexpr (C::kChunk == 32) tmem_ld32(ta, v);
                     else tmem_ld16(ta, v);
                 }
@@ -259,21 +690,113 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, 1)
                 }
                 const int cnt = (int)min((int64_t)C::kChunk, p.m - tok);
                 if (cnt <= 0) continue;
-                if (lane < C::kChunk) sc[lane] = lane < cnt ? (ok ? p.a_scale[tok + lane] : __int_as_float(0x7fffffff)) : 0.f;
+                if (lane < cnt) sc[lane] = ok ? p.a_scale[tok + lane] : __int_as_float(0x7fffffff);
                 __syncwarp();
-                T* o = out + tok * p.ldo + ch;
-                if (in) {
-#pragma unroll
-                    for (int j = 0; j < C::kChunk; ++j) {
-                        if (j < cnt) mm_emit(o, (int)v[j], sc[j], sb, bias);
-                        o += p.ldo;
-                    }
+                mm_block(q, tok * p.ldo + ch, v, sc, cnt, sb, bias, (int)min((int64_t)32, p.n - (ch - lane)), lane);
+                __syncwarp();
+            }
+        }
+    } else if constexpr (!TMA) {
+        // Groups of 4 warps take the stages in turn, so that one group's loads, stores and fence overlap the
+        // others' (all 16 warps on every stage took twice as long).  A thread loads 16 bytes, chunk c, of the rows
+        // r0, r0 + 16, ..., four at a time.
+        constexpr int kGroups = C::kLoad / 4, kPer = (kMmM + NT) / 16;
+        static_assert(kPer % 4 == 0 && kMmM % 64 == 0, "four rows at a time are of one operand");
+        const int lt = tid - 64 - 32 * C::kEpi, r0 = (lt & 127) >> 3, c = lt & 7;
+        const uint32_t group = (uint32_t)lt >> 7;
+        const uintptr_t b_lo = reinterpret_cast<uintptr_t>(p.b), b_hi = b_lo + (p.n - 1) * p.ldb + p.k;
+        const uintptr_t a_lo = reinterpret_cast<uintptr_t>(p.a), a_hi = a_lo + (p.m - 1) * p.lda + p.k;
+        uint32_t i = 0;                                          // stages of all groups so far
+        bool ok = true;
+        for (uint32_t t = t0; ok && t < tiles; t += gridDim.x) {
+            int ct, tt;
+            mm_place(t, q.tn, q.tm, ct, tt);
+            for (int kb = kb0; kb < kb1; ++kb, ++i) {
+                if (i % kGroups != group) continue;
+                const uint32_t s = i % C::kStages, lap = i / C::kStages;
+                if (lap > 0) ok = __all_sync(0xffffffffu, mm_wait(&bar_empty[s], (lap - 1) & 1, vfail));
+                if (!ok) {
+                    if (lane == 0) s_fail = 1;
+                    break;
                 }
+                unsigned char* st = sm + (size_t)s * C::kStage + r0 * 128 + ((c ^ (r0 & 7)) << 4);
+                // no load of this step leaves its row by more than the 16-byte pieces around it, nor the arrays
+                const bool inner = (kb + 1) * kMmK + 16 <= p.k && ((a_lo | b_lo) & 15) == 0;
+#pragma unroll 1
+                for (int u0 = 0; u0 < kPer; u0 += 4) {
+                    const bool is_b = u0 * 16 < kMmM;
+                    const uintptr_t lo = is_b ? b_lo : a_lo, hi = is_b ? b_hi : a_hi;
+                    const int64_t ld = is_b ? p.ldb : p.lda, rows = is_b ? p.n : p.m;
+                    const int64_t row = (is_b ? (int64_t)ct * kMmM : (int64_t)tt * NT - kMmM) + r0 + u0 * 16;
+                    MmBytes<false> raw[4];
+                    uintptr_t at[4], end[4];                     // a row past the last one is empty
+                    if (inner && row - r0 + 64 <= rows) {
+                        const uintptr_t first = lo + row * ld + kb * kMmK + 16 * c;
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) raw[u].issue_inside(first + u * 16 * ld);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            *reinterpret_cast<uint4*>(st + (u0 + u) * 16 * 128) = raw[u].shifted(first + u * 16 * ld);
+                        continue;
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const bool in = row + u * 16 < rows;
+                        const uintptr_t first = lo + (in ? row + u * 16 : 0) * ld;
+                        at[u] = first + kb * kMmK + 16 * c;
+                        end[u] = in ? first + p.k : 0;
+                        raw[u].issue(at[u], end[u], lo, hi);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        *reinterpret_cast<uint4*>(st + (u0 + u) * 16 * 128) = raw[u].take(at[u], end[u], lo, hi);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_full[s]);
             }
         }
     }
 
+    __syncthreads();
+    if (split > 1) {
+        // every part's sums are in its shared memory; column c of the tile falls to part c % split
+        cluster_sync();
+        int ct, tt;
+        mm_place(t0, q.tn, q.tm, ct, tt);
+        const int bad = s_fail;
+        const uint32_t x = smem_u32(sm), fail_at = smem_u32(&s_fail);
+        int any = bad;
+        for (int r = 0; r < split; ++r) any |= cluster_load(fail_at, r);
+        const int64_t left = p.m - (int64_t)tt * NT;
+        const int cols = (int)(left < NT ? left : NT);
+        for (int e = tid; e < kMmM / 4 * ((cols - part + split - 1) / split); e += C::kThreads) {
+            const int c = part + e / (kMmM / 4) * split, l = e % (kMmM / 4) * 4;      // 4 channels of column c
+            int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 4
+            for (int r = 0; r < split; ++r) {
+                const int4 v = cluster_load4(x + 4u * (uint32_t)(c * kMmM + l), r);
+                sum.x += v.x;
+                sum.y += v.y;
+                sum.z += v.z;
+                sum.w += v.w;
+            }
+            const int64_t ch = (int64_t)ct * kMmM + l, tok = (int64_t)tt * NT + c;
+            const float sa = any ? __int_as_float(0x7fffffff) : p.a_scale[tok];
+            const int part_sum[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (ch + i >= p.n) break;
+                const float sb = p.b_scale[ch + i], bias = p.bias ? p.bias[ch + i] : 0.f;
+                const int64_t at = tok * p.ldo + ch + i;
+                if (q.out_type == kSqF32) mm_emit(static_cast<float*>(p.out) + at, part_sum[i], sa, sb, bias);
+                else if (q.out_type == kSqF16) mm_emit(static_cast<__half*>(p.out) + at, part_sum[i], sa, sb, bias);
+                else mm_emit(static_cast<__nv_bfloat16*>(p.out) + at, part_sum[i], sa, sb, bias);
+            }
+        }
+        __syncthreads();
+        cluster_sync();                                          // no CTA leaves while its sums are read
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -281,8 +804,8 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kCols) : "memory");
 }
 
-// the tensor map of int8 rows [n, k], ld bytes apart, read by boxes of 128 bytes x `box` rows
-cudaError_t mm_map(const int8_t* rows, int64_t n, int k, int64_t ld, int box, CUtensorMap* map) {
+// the tensor map of int8 rows [n, k], ld bytes apart, in swizzled boxes of 128 bytes x `box` rows
+cudaError_t mm_map_rows(const int8_t* rows, int64_t n, int k, int64_t ld, int box, CUtensorMap* map) {
     using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                        const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                        CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -298,65 +821,146 @@ cudaError_t mm_map(const int8_t* rows, int64_t n, int k, int64_t ld, int box, CU
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-int sm_count() {
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms;
-}
+// whether 2 neighbouring 16-bit outputs of a row may be stored at once
+bool pair_out(const SqMatmul& p, int out_type) { return out_type != kSqF32 && rows_aligned(p.out, 2 * p.ldo, 4); }
 
-template <typename T, int NT>
-cudaError_t launch_tc(const SqMatmul& p, cudaStream_t st) {
-    using C = MmCfg<NT>;
-    CUtensorMap map_b, map_a;
-    cudaError_t e = mm_map(p.b, p.n, p.k, p.ldb, kMmM, &map_b);
-    if (!e) e = mm_map(p.a, p.m, p.k, p.lda, NT, &map_a);
-    if (!e) e = cudaFuncSetAttribute(mm_tc_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
+template <int NT, bool TMA>
+cudaError_t go_tc(const SqMatmul& p, int out_type, int split, cudaStream_t st) {
+    using C = MmCfg<NT, TMA>;
+    CUtensorMap map_b{}, map_a{};
+    cudaError_t e = cudaSuccess;
+    if (TMA) {
+        e = mm_map_rows(p.b, p.n, p.k, p.ldb, kMmM, &map_b);
+        if (!e) e = mm_map_rows(p.a, p.m, p.k, p.lda, NT, &map_a);
+    }
+    if (!e) e = cudaFuncSetAttribute(mm_tc_kernel<NT, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
     if (e) return e;
-    const int tn = (int)((p.n + kMmM - 1) / kMmM), tm = (int)((p.m + NT - 1) / NT);
-    const int grid = (int)std::min<int64_t>((int64_t)tn * tm, sm_count());
+    MmTc q{};
+    q.p = p;
+    q.out_type = out_type;
+    q.pair = pair_out(p, out_type);
+    q.tn = (uint32_t)((p.n + kMmM - 1) / kMmM);
+    q.tm = (uint32_t)((p.m + NT - 1) / NT);
+    if ((int64_t)q.tn * q.tm >= int64_t(1) << 31) return cudaErrorInvalidValue;
+    const int kb = (p.k + kMmK - 1) / kMmK;
+    q.kb_part = (kb + split - 1) / split;
+    q.split = (kb + q.kb_part - 1) / q.kb_part == split ? split : 1;     // every part has work
+    if (q.split == 1) q.kb_part = kb;
+    const int64_t tiles = (int64_t)q.tn * q.tm;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(q.split > 1 ? tiles * q.split : std::min<int64_t>(tiles, (int64_t)sm_count() * C::kCtas)));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)q.split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
     note_launch();
-    mm_tc_kernel<T, NT><<<grid, C::kThreads, C::kSmem, st>>>(map_b, map_a, p, tn, tm);
-    return cudaGetLastError();
+    return cudaLaunchKernelEx(&cfg, mm_tc_kernel<NT, TMA>, map_b, map_a, q);
 }
 
-bool rows_aligned(const void* p, int64_t ld, int a) { return reinterpret_cast<uintptr_t>(p) % a == 0 && ld % a == 0; }
+// Which tile and how many parts of k: the least of an estimate, in us, that was
+// fitted to sweeps of 30 shapes from 16 x 512 x 8192 to 256 x 1M x 128 on a B200
+// (the choice is within 10 % of the best of each sweep).  An SM draws what it
+// has in flight per 1.6 us of latency under load, whole stages of its resident
+// CTAs; b comes from HBM at 5 TB/s or from L2; a unit's epilogue costs 0.35 us
+// and 1 us per 13000 outputs; a split costs a cluster launch, two cluster barriers and the
+// sums' way through shared memory, and CTAs beyond those that are resident start anew.
+// With few tiles a split is worth much: 64 x 256 x 16384 takes 11.3 us in 8
+// parts, 46 us whole; 256 x 4096 x 4096 14.9 and 17.3 us.
+struct MmPick {
+    int nt, split;
+    double us;
+};
 
-template <typename T>
-cudaError_t launch_mm(const SqMatmul& p, cudaStream_t st) {
-    if (rows_aligned(p.a, p.lda, 16) && rows_aligned(p.b, p.ldb, 16)) {
-        if (p.m <= 16) return launch_tc<T, 16>(p, st);
-        if (p.m <= 32) return launch_tc<T, 32>(p, st);
-        if (p.m <= 64) return launch_tc<T, 64>(p, st);
-        if (p.m <= 128) return launch_tc<T, 128>(p, st);
-        return launch_tc<T, 256>(p, st);
+template <int NT, bool TMA>
+void mm_estimate(const SqMatmul& p, int sms, MmPick& best) {
+    using C = MmCfg<NT, TMA>;
+    if (NT > (TMA ? 16 : 64) && NT / 2 >= p.m) return;           // a smaller tile holds all tokens
+    const double tm = (double)((p.m + NT - 1) / NT), tiles = (double)((p.n + kMmM - 1) / kMmM) * tm;
+    const int kb = (p.k + kMmK - 1) / kMmK;
+    const double rows = kMmM + std::min<int64_t>(NT, p.m), epi = 0.35 + NT * kMmM / 13000.0;
+    for (int split = 1; split <= 8; split *= 2) {
+        if (split > 1 && (kb < 2 * split || tiles * split > 8.0 * sms)) break;
+        const double per_sm = std::ceil(tiles * split / sms);
+        const double flight = std::min<double>(C::kCtas, per_sm) * C::kStage * C::kStages;
+        const double rate = TMA ? flight / 1.6e3 : 25.0;         // bytes a ns
+        const double part = (kb + split - 1) / split * (double)kMmK;
+        double us = std::max(per_sm * rows * part / rate / 1e3, (double)p.n * p.k / 5e6);
+        us = 4.0 + std::max(us, per_sm * epi) + epi;
+        if (split > 1) us += 1.6 + 0.01 * NT + 3.0 * (std::ceil(tiles * split / (sms * C::kCtas)) - 1);
+        us *= 1.0 + 0.05 * std::min<double>(4.0, tm - 1.0);      // every token tile reads b again
+        if (us < best.us) best = {NT, split, us};
     }
-    const int64_t tiles_n = (p.n + kTile - 1) / kTile, tiles_m = (p.m + kTile - 1) / kTile;
-    // a grid holds 2^31 - 1 blocks: more tiles go in several launches of whole tile rows
-    const int64_t per = std::max<int64_t>(1, ((int64_t(1) << 31) - 1) / tiles_n);
-    for (int64_t r = 0; r < tiles_m; r += per) {
-        SqMatmul q = p;
-        q.a = p.a + r * kTile * p.lda;
-        q.a_scale = p.a_scale + r * kTile;
-        q.out = static_cast<T*>(p.out) + r * kTile * p.ldo;
-        q.m = std::min<int64_t>(p.m - r * kTile, per * kTile);
-        const int64_t rows = (q.m + kTile - 1) / kTile;
-        note_launch();
-        mm_tile_kernel<T><<<(unsigned)(rows * tiles_n), 256, 0, st>>>(
-            q, rows_aligned(q.a, q.lda, 4), rows_aligned(q.b, q.ldb, 4), (int)tiles_n);
-        const cudaError_t e = cudaGetLastError();
-        if (e) return e;
+}
+
+cudaError_t launch_tc(const SqMatmul& p, int out_type, cudaStream_t st) {
+    MmPick pick{0, 1, 1e300};
+    const int sms = sm_count();
+    if (!rows_aligned(p.a, p.lda, 16) || !rows_aligned(p.b, p.ldb, 16)) {
+        mm_estimate<64, false>(p, sms, pick);
+        mm_estimate<128, false>(p, sms, pick);
+        return pick.nt == 64 ? go_tc<64, false>(p, out_type, pick.split, st)
+                             : go_tc<128, false>(p, out_type, pick.split, st);
     }
-    return cudaSuccess;
+    mm_estimate<16, true>(p, sms, pick);
+    mm_estimate<32, true>(p, sms, pick);
+    mm_estimate<64, true>(p, sms, pick);
+    mm_estimate<128, true>(p, sms, pick);
+    mm_estimate<256, true>(p, sms, pick);
+    switch (pick.nt) {
+        case 16: return go_tc<16, true>(p, out_type, pick.split, st);
+        case 32: return go_tc<32, true>(p, out_type, pick.split, st);
+        case 64: return go_tc<64, true>(p, out_type, pick.split, st);
+        case 128: return go_tc<128, true>(p, out_type, pick.split, st);
+        default: return go_tc<256, true>(p, out_type, pick.split, st);
+    }
 }
 
 }  // namespace
 
 cudaError_t sq_matmul(const SqMatmul& p, int out_type, cudaStream_t st) {
     if (p.m == 0 || p.n == 0) return cudaSuccess;
-    if (out_type == kSqF32) return launch_mm<float>(p, st);
-    if (out_type == kSqF16) return launch_mm<__half>(p, st);
-    return launch_mm<__nv_bfloat16>(p, st);
+    // one token, or a few where the tensor-core kernel would have to put its rows together: dot products
+    const bool aligned = rows_aligned(p.a, p.lda, 16) && rows_aligned(p.b, p.ldb, 16);
+    if (dot_usable(p) && (p.m == 1 || !aligned)) {
+        MmDot q{};
+        q.p = p;
+        q.out_type = out_type;
+        return launch_dot(q, st);
+    }
+    return launch_tc(p, out_type, st);
+}
+
+bool sq_scores_fused(int64_t m, int k) {
+    SqMatmul p{};
+    p.m = m;
+    p.k = k;
+    return dot_usable(p);
+}
+
+cudaError_t sq_scores(const SqWrite& w, int x_type, SqMatmul p, int out_type, cudaStream_t st) {
+    if (p.m == 0 || p.n == 0) return cudaSuccess;
+    if (dot_usable(p)) {
+        MmDot q{};
+        q.p = p;
+        q.x = w.x;
+        q.ldx = w.ldx;
+        q.x_type = x_type;
+        q.out_type = out_type;
+        const int es = x_type == kSqF32 ? 4 : 2;
+        q.x_vec = rows_aligned(w.x, (int64_t)w.ldx * es, 16) && (p.k * es) % 16 == 0;
+        return launch_dot(q, st);
+    }
+    const cudaError_t e = sq_write(w, x_type, 8, st);
+    if (e) return e;
+    p.a = reinterpret_cast<const int8_t*>(w.codes);
+    p.a_scale = w.scales;
+    p.lda = w.ldc;
+    return sq_matmul(p, out_type, st);
 }
 
 }  // namespace isb

@@ -908,10 +908,10 @@ class SQRows:
         to = _sq_type(dtype)
         out, ldo = _sq_out(out, m, self.capacity, dtype, self.device)
         need = self.L.ivf_sq_scores_work(m, self.d)
-        work = torch.empty(need, dtype=torch.uint8, device=self.device)
+        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         _sq_call(self.L.ivf_sq_scores, self.device, x.data_ptr(), t, ldx, m, self._codes.data_ptr(), self._ldc,
                  self._scales.data_ptr(), self.capacity, self.d, None if bias is None else bias.data_ptr(), out.data_ptr(),
-                 to, ldo, work.data_ptr(), need)
+                 to, ldo, None if work is None else work.data_ptr(), need)
         return out
 
 

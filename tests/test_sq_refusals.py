@@ -19,7 +19,7 @@ READ = dict(codes=P, ldc=32, scales=P, lds=1, capacity=16, bits=8, group=0, slot
             ldo=32, stream=None)
 MATMUL = dict(a=P, lda=32, a_scale=P, m=4, b=P, ldb=32, b_scale=P, n=8, k=32, bias=None, out=P, out_type=0, ldo=8,
               stream=None)
-SCORES = dict(x=P, x_type=0, ldx=32, m=4, codes=P, ldc=32, scales=P, n=8, d=32, bias=None, out=P, out_type=0, ldo=8,
+SCORES = dict(x=P, x_type=0, ldx=32, m=8, codes=P, ldc=32, scales=P, n=8, d=32, bias=None, out=P, out_type=0, ldo=8,
               work=P, work_bytes=1 << 20, stream=None)
 
 
@@ -33,8 +33,8 @@ def call(name, base, **change):
     dict(x_type=3), dict(x_type=-1), dict(n=-1), dict(n=1 << 31), dict(d=0), dict(d=(1 << 20) + 1), dict(ldx=31),
     dict(x=None), dict(x=P + 2), dict(x_type=1, x=P + 1), dict(bits=2), dict(bits=16), dict(group=-16),
     dict(group=8), dict(group=24), dict(codes=None), dict(scales=None), dict(scales=P + 2), dict(ldc=31),
-    dict(bits=4, ldc=15), dict(group=16, lds=1), dict(capacity=-1), dict(slots=None, n=17), dict(slots=P + 4),
-    dict(n=513, capacity=1000, claim=None), dict(n=513, capacity=1000, claim=P + 2)])
+    dict(bits=4, ldc=15), dict(group=16, lds=1), dict(capacity=-1), dict(capacity=1 << 31),
+    dict(slots=None, n=17), dict(slots=P + 4), dict(ldx=1 << 32), dict(n=513, capacity=1000, claim=None), dict(n=513, capacity=1000, claim=P + 2)])
 def test_write_refuses(change):
     rc, msg = call("ivf_sq_write", WRITE, **change)
     assert rc == EINVAL and msg
@@ -62,7 +62,7 @@ def test_matmul_refuses(change):
 @pytest.mark.parametrize("change", [
     dict(x_type=3), dict(ldx=31), dict(m=-1), dict(n=-1), dict(d=0), dict(d=131072), dict(ldc=31), dict(ldo=7),
     dict(x=None), dict(codes=None), dict(scales=None), dict(out=None), dict(work=None), dict(work=P + 8),
-    dict(work_bytes=4 * 32 + 4 * 4 - 1)])
+    dict(work_bytes=8 * 32 + 4 * 8 - 1)])
 def test_scores_refuses(change):
     rc, msg = call("ivf_sq_scores", SCORES, **change)
     assert rc == EINVAL and msg
@@ -84,6 +84,7 @@ def test_scores_work():
     assert L.ivf_sq_scores_work(10, 97) >= 10 * (112 + 4)
     assert L.ivf_sq_scores_work((1 << 31) - 2, 131071) >= ((1 << 31) - 2) * (131072 + 4)
     assert L.ivf_sq_scores_work(-1, 8) == L.ivf_sq_scores_work(8, 0) == L.ivf_sq_scores_work(8, 131072) == 0
+    assert L.ivf_sq_scores_work(1, 96) == L.ivf_sq_scores_work(0, 96) == 0     # nothing to keep between two kernels
 
 
 def test_binding_refuses_without_a_device():
