@@ -370,24 +370,28 @@ int ivf_sq_read(const void* d_codes, long long ldc, const float* d_scales, long 
  * a [m, k], b [n, k] int8 (any value), rows lda and ldb bytes apart; scales
  * and bias (may be NULL) fp32, dense; out [m, n] of out_type, rows ldo values
  * apart.  The sum is exact (1 <= k <= IVF_SQ_MAX_K); the rest is fp32, rounded
- * once to out_type.  m, n < 2^31.
+ * once to out_type.  m, n < 2^31.  d_work: scratch of ivf_sq_matmul_work()
+ * bytes, 16-byte aligned, for operands whose rows are not 16-byte aligned (0
+ * bytes, and it may be NULL, where they are and for a few tokens).
  */
 int ivf_sq_matmul(const int8_t* d_a, long long lda, const float* d_a_scale, long long m, const int8_t* d_b,
                   long long ldb, const float* d_b_scale, long long n, int k, const float* d_bias, void* d_out,
-                  int out_type, long long ldo, void* stream);
+                  int out_type, long long ldo, void* d_work, size_t work_bytes, void* stream);
+/* bytes of d_work that ivf_sq_matmul needs for these arrays (0 for sizes that it refuses) */
+size_t ivf_sq_matmul_work(const int8_t* d_a, long long lda, long long m, const int8_t* d_b, long long ldb, long long n,
+                          int k);
 /*
- * Scores of floating tokens against n rows of an 8-bit store with one scale a row: d_x [m, d]
- * (x_type, rows ldx values apart) is quantised as ivf_sq_write does (bits 8,
- * group 0), then multiplied as by ivf_sq_matmul, with equal results.
- * d_scales dense [n].  d_work: scratch of ivf_sq_scores_work(m, d) bytes,
- * 16-byte aligned (may be NULL where that is 0).
+ * Scores of floating tokens against n rows of an 8-bit store with one scale a
+ * row: d_x [m, d] (x_type, rows ldx values apart) is quantised as ivf_sq_write
+ * does (bits 8, group 0), then multiplied as by ivf_sq_matmul, with equal
+ * results.  d_scales dense [n].  d_work: scratch of ivf_sq_scores_work() bytes,
+ * 16-byte aligned (may be NULL where that is 0: for a few tokens).
  */
 int ivf_sq_scores(const void* d_x, int x_type, long long ldx, long long m, const int8_t* d_codes, long long ldc,
                   const float* d_scales, long long n, int d, const float* d_bias, void* d_out, int out_type,
                   long long ldo, void* d_work, size_t work_bytes, void* stream);
-/* bytes of d_work that ivf_sq_scores needs: 0 for a few tokens (and for sizes
- * that it refuses) */
-size_t ivf_sq_scores_work(long long m, int d);
+/* bytes of d_work that ivf_sq_scores needs for this store (0 for sizes that it refuses) */
+size_t ivf_sq_scores_work(long long m, const int8_t* d_codes, long long ldc, long long n, int d);
 
 /* ======================================================================
  * Update overlay (new: runner-internal in the reference,

@@ -1483,8 +1483,10 @@ SqMatmul sq_check_product(const int8_t* b, long long ldb, const float* b_scale, 
     p.ldo = ldo;
     return p;
 }
-// row stride of the quantised tokens in ivf_sq_scores' scratch
-long long sq_work_ld(int d) { return (d + 15ll) / 16 * 16; }
+void sq_check_work(const void* work, size_t bytes, size_t needed) {
+    need(needed == 0 || (work && bytes >= needed), "d_work is smaller than the call needs");
+    need(reinterpret_cast<uintptr_t>(work) % 16 == 0, "d_work must be 16-byte aligned");
+}
 }  // namespace
 
 int ivf_sq_write(const void* d_x, int x_type, long long n, int d, long long ldx, const long long* d_slots, int bits,
@@ -1542,7 +1544,7 @@ int ivf_sq_read(const void* d_codes, long long ldc, const float* d_scales, long 
 
 int ivf_sq_matmul(const int8_t* d_a, long long lda, const float* d_a_scale, long long m, const int8_t* d_b,
                   long long ldb, const float* d_b_scale, long long n, int k, const float* d_bias, void* d_out,
-                  int out_type, long long ldo, void* stream) {
+                  int out_type, long long ldo, void* d_work, size_t work_bytes, void* stream) {
     return guarded(nullptr, [&] {
         need(m >= 0 && m < 2147483647ll, "need 0 <= m < 2^31 - 1");
         SqMatmul p = sq_check_product(d_b, ldb, d_b_scale, m, n, k, d_bias, d_out, out_type, ldo);
@@ -1552,14 +1554,25 @@ int ivf_sq_matmul(const int8_t* d_a, long long lda, const float* d_a_scale, long
         p.a = d_a;
         p.a_scale = d_a_scale;
         p.lda = lda;
+        sq_check_work(d_work, work_bytes, sq_matmul_work(p));
         if (m == 0 || n == 0) return;
-        ck(sq_matmul(p, out_type, static_cast<cudaStream_t>(stream)), "sq_matmul");
+        ck(sq_matmul(p, out_type, d_work, static_cast<cudaStream_t>(stream)), "sq_matmul");
     });
 }
 
-size_t ivf_sq_scores_work(long long m, int d) {
-    if (m <= 0 || m >= 2147483647ll || d < 1 || d > IVF_SQ_MAX_K || sq_scores_fused(m, d)) return 0;
-    return (size_t)m * (size_t)(sq_work_ld(d) + 4) + 16;
+size_t ivf_sq_matmul_work(const int8_t* d_a, long long lda, long long m, const int8_t* d_b, long long ldb, long long n,
+                          int k) {
+    if (m <= 0 || m >= 2147483647ll || n <= 0 || n >= 2147483647ll || k < 1 || k > IVF_SQ_MAX_K || lda < k || ldb < k)
+        return 0;
+    SqMatmul p{};
+    p.a = d_a;
+    p.lda = lda;
+    p.m = m;
+    p.b = d_b;
+    p.ldb = ldb;
+    p.n = n;
+    p.k = k;
+    return sq_matmul_work(p);
 }
 
 int ivf_sq_scores(const void* d_x, int x_type, long long ldx, long long m, const int8_t* d_codes, long long ldc,
@@ -1569,22 +1582,26 @@ int ivf_sq_scores(const void* d_x, int x_type, long long ldx, long long m, const
         need(d >= 1 && d <= IVF_SQ_MAX_K, "need 1 <= d <= IVF_SQ_MAX_K");
         sq_check_rows(d_x, x_type, m, d, ldx, "x");
         SqMatmul p = sq_check_product(d_codes, ldc, d_scales, m, n, d, d_bias, d_out, out_type, ldo);
-        const size_t work = ivf_sq_scores_work(m, d);
-        need(work == 0 || (d_work && work_bytes >= work), "d_work is smaller than ivf_sq_scores_work(m, d)");
-        need(reinterpret_cast<uintptr_t>(d_work) % 16 == 0, "d_work must be 16-byte aligned");
+        sq_check_work(d_work, work_bytes, sq_scores_work(p));
         if (m == 0 || n == 0) return;
         SqWrite w{};
         w.x = d_x;
         w.n = (uint32_t)m;
         w.ldx = (uint32_t)ldx;
         w.d = d;
-        w.codes = static_cast<uint8_t*>(d_work);
-        w.ldc = (uint32_t)sq_work_ld(d);
-        w.scales = reinterpret_cast<float*>(w.codes + (size_t)m * w.ldc);
-        w.lds = 1;
-        w.capacity = (uint32_t)m;
-        ck(sq_scores(w, x_type, p, out_type, static_cast<cudaStream_t>(stream)), "sq_scores");
+        ck(sq_scores(w, x_type, p, out_type, d_work, static_cast<cudaStream_t>(stream)), "sq_scores");
     });
+}
+
+size_t ivf_sq_scores_work(long long m, const int8_t* d_codes, long long ldc, long long n, int d) {
+    if (m <= 0 || m >= 2147483647ll || n <= 0 || n >= 2147483647ll || d < 1 || d > IVF_SQ_MAX_K || ldc < d) return 0;
+    SqMatmul p{};
+    p.m = m;
+    p.b = d_codes;
+    p.ldb = ldc;
+    p.n = n;
+    p.k = d;
+    return sq_scores_work(p);
 }
 
 int ivf_set_shard(void* idx_ctx, int nlist_global, const int* local_to_global, const long long* key_offsets) {

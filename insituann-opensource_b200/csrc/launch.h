@@ -266,11 +266,12 @@ struct SqMatmul {
     void* out;                   // [m, n], ldo apart
     int64_t ldo;
 };
-cudaError_t sq_matmul(const SqMatmul& p, int out_type, cudaStream_t st);
-// the product of the floating rows of w (x_type), quantised one scale a row
-// into w's codes and scales (or by the product itself); p without its tokens but for m
-cudaError_t sq_scores(const SqWrite& w, int x_type, SqMatmul p, int out_type, cudaStream_t st);
-// whether the product of m tokens quantises them itself (w's codes and scales are not used)
-bool sq_scores_fused(int64_t m, int k);
+// work: sq_matmul_work(p) bytes, 16-byte aligned (for rows that are not)
+size_t sq_matmul_work(const SqMatmul& p);
+cudaError_t sq_matmul(SqMatmul p, int out_type, void* work, cudaStream_t st);
+// the product of the floating rows of w (x_type; only x, n, ldx, d are given),
+// quantised one scale a row; p without its tokens but for m
+size_t sq_scores_work(const SqMatmul& p);
+cudaError_t sq_scores(SqWrite w, int x_type, SqMatmul p, int out_type, void* work, cudaStream_t st);
 
 }  // namespace isb

@@ -1,5 +1,16 @@
-// sq.cuh -- device building blocks of the scalar-quantised rows, shared by sq.cu
-// (write, read) and sq_mm.cu (the product that quantises its own tokens).
+// sq.cuh -- device building blocks of the scalar-quantised rows, shared by
+// sq_write.cu, sq_read.cu and sq_mm.cu (whose product quantises few tokens itself).
+//
+// For a group of values x (the whole row, or `group` consecutive values; the
+// last group of a row may be shorter) and L = 127 (8 bits) or 7 (4 bits):
+//     scale = fp32(max |x| / L)
+//     code  = the whole number nearest to x / scale (ties to even), in [-L, L];
+//             0 where the scale is 0
+//     value = code * scale in fp32, rounded to the type it is read in.
+// The scale is kept in fp32: 4 bytes a group, and an error of 2^-24 next to the
+// half step (2^-8 of the group's largest value at 8 bits) that the code costs.
+// A group with a NaN or an infinity keeps that NaN or infinity as its scale
+// and codes of 0, so it reads back as NaN.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -17,12 +28,27 @@ __device__ __forceinline__ void sq_round(float v, float& o) { o = v; }
 __device__ __forceinline__ void sq_round(float v, __half& o) { o = __float2half_rn(v); }
 __device__ __forceinline__ void sq_round(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 
-// Values per chunk: 16 bytes of the floating type where rows are 16-byte aligned
-// and a whole number of chunks long (VEC), else the fewest that fill a byte of
-// codes.  With VEC a chunk is inside its group or outside, so nothing below handles a part of one.
-template <typename T, int BITS, bool VEC>
+// How floating rows are taken, a chunk at a time:
+//   kSqVec      rows are 16-byte aligned and a whole number of chunks of 16 bytes
+//               long: a chunk is inside its group or outside
+//   kSqShifted  rows of any alignment, in chunks of 16 bytes put together from
+//               aligned pieces; a group's last chunk may be a part (the codes
+//               are aligned as for kSqVec)
+//   kSqSingle   chunks of the fewest values that fill a byte of codes
+constexpr int kSqSingle = 0, kSqVec = 1, kSqShifted = 2;
+
+template <typename T, int BITS, int MODE>
 __host__ __device__ constexpr int sq_chunk() {
-    return VEC ? 16 / (int)sizeof(T) : 8 / BITS;
+    return MODE != kSqSingle ? 16 / (int)sizeof(T) : 8 / BITS;
+}
+
+constexpr uint32_t kNoSlot = 0xffffffffu;
+
+// slot of a row, kNoSlot outside the store
+__device__ __forceinline__ uint32_t sq_slot(const long long* __restrict__ slots, uint32_t row, uint32_t capacity) {
+    if (!slots) return row;
+    const unsigned long long s = (unsigned long long)slots[row];
+    return s < capacity ? (uint32_t)s : kNoSlot;
 }
 
 // item = row * parts + part
@@ -65,6 +91,87 @@ __device__ __forceinline__ float2 sq_mul2(float2 a, float2 b) {
     return d;
 }
 
+// 16 bytes of a row in flight: issue() starts the loads and has no branch, so
+// that several of them are under way at once; take() gives the bytes.  ALIGNED:
+// rows are 16-byte aligned, and what follows a row's end is what lies there;
+// else the two aligned 16-byte pieces around the bytes are read and shifted, and
+// 0 follows a row's end.  A piece that is not wholly inside the array [lo, hi)
+// (at its ends only) is read by bytes.
+template <bool ALIGNED>
+struct SqBytes {
+    uint32_t v[ALIGNED ? 4 : 8];
+
+    // bytes [at, at + 16) of a row that ends at `end` (at >= end: none)
+    __device__ __forceinline__ void issue(uintptr_t at, uintptr_t end, uintptr_t lo, uintptr_t hi) {
+        if constexpr (ALIGNED) {
+            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+            if (at < end && at + 16 <= hi) x = __ldg(reinterpret_cast<const uint4*>(at));
+            v[0] = x.x;
+            v[1] = x.y;
+            v[2] = x.z;
+            v[3] = x.w;
+        } else {
+            const uintptr_t w = at & ~uintptr_t(15);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                if (at < end && w + 16 * h < end && w + 16 * h >= lo && w + 16 * h + 16 <= hi)
+                    x = __ldg(reinterpret_cast<const uint4*>(w + 16 * h));
+                v[4 * h] = x.x;
+                v[4 * h + 1] = x.y;
+                v[4 * h + 2] = x.z;
+                v[4 * h + 3] = x.w;
+            }
+        }
+    }
+    __device__ __forceinline__ uint4 take(uintptr_t at, uintptr_t end, uintptr_t lo, uintptr_t hi) {
+        if constexpr (ALIGNED) {
+            if (at < end && at + 16 > hi) {                      // the last bytes of the array
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = edge(at + 4 * i, lo, hi);
+            }
+            return make_uint4(v[0], v[1], v[2], v[3]);
+        } else {
+            const uintptr_t w = at & ~uintptr_t(15);
+            if (at < end && (w < lo || w + 32 > hi)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (w + (i & 4) * 4 < lo || w + (i & 4) * 4 + 16 > hi) v[i] = edge(w + 4 * i, lo, hi);
+            }
+            const uint4 x = shifted(at);
+            uint32_t o[4] = {x.x, x.y, x.z, x.w};
+            if (at + 16 > end) {                                 // clear what follows the row
+                const int left = at < end ? (int)(end - at) : 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int n = left - 4 * i;
+                    o[i] = n >= 4 ? o[i] : n <= 0 ? 0u : o[i] & ((1u << (8 * n)) - 1u);
+                }
+            }
+            return make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+    // the 16 bytes from at & 15 on: by two words, by one, by bits
+    __device__ __forceinline__ uint4 shifted(uintptr_t at) {
+        const bool two = (at & 8) != 0, one = (at & 4) != 0;
+#pragma unroll
+        for (int i = 0; i < 6; ++i) v[i] = two ? v[i + 2] : v[i];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) v[i] = one ? v[i + 1] : v[i];
+        const uint32_t sh = (uint32_t)(at & 3) * 8;
+        return make_uint4(__funnelshift_r(v[0], v[1], sh), __funnelshift_r(v[1], v[2], sh),
+                          __funnelshift_r(v[2], v[3], sh), __funnelshift_r(v[3], v[4], sh));
+    }
+    // the word at w, 0 where its bytes are outside [lo, hi)
+    static __device__ __forceinline__ uint32_t edge(uintptr_t w, uintptr_t lo, uintptr_t hi) {
+        uint32_t x = 0;
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i)
+            if (w + i >= lo && w + i < hi) x |= (uint32_t)*reinterpret_cast<const uint8_t*>(w + i) << (8 * i);
+        return x;
+    }
+};
+
 // ---- floating chunks, kept as they were read (half the registers of fp32 for
 // the 16-bit types) ----
 template <typename T, int E>
@@ -88,27 +195,44 @@ struct SqRaw {
     }
 };
 
-// values e0 .. e0 + E - 1 of a group of `width` values, 0 past its end
-template <typename T, bool VEC, int E>
-__device__ __forceinline__ SqRaw<T, E> sq_load(const T* __restrict__ x, int e0, int width) {
+// Values e0 .. e0 + E - 1 of a group of `width` values at x, 0 past its end:
+// issue() starts the loads, take() gives the values.  [lo, hi): all the rows' bytes.
+template <typename T, int MODE, int E>
+struct SqLoad {
     SqRaw<T, E> r;
+    __device__ __forceinline__ void issue(const T* __restrict__ x, int e0, int width, uintptr_t, uintptr_t) {
 #pragma unroll
-    for (int i = 0; i < SqRaw<T, E>::kWords; ++i) r.w[i] = 0;
-    if constexpr (VEC) {
-        if (e0 < width) {
-            const uint4 v = *reinterpret_cast<const uint4*>(x + e0);
-            memcpy(r.w, &v, sizeof(r.w));
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (e0 + e < width) {
-                if constexpr (sizeof(T) == 4) r.w[e] = reinterpret_cast<const uint32_t*>(x)[e0 + e];
-                else r.w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(x)[e0 + e] << (16 * (e & 1));
+        for (int i = 0; i < SqRaw<T, E>::kWords; ++i) r.w[i] = 0;
+        if constexpr (MODE == kSqVec) {
+            if (e0 < width) {
+                const uint4 v = *reinterpret_cast<const uint4*>(x + e0);
+                memcpy(r.w, &v, sizeof(r.w));
             }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e0 + e < width) {
+                    if constexpr (sizeof(T) == 4) r.w[e] = reinterpret_cast<const uint32_t*>(x)[e0 + e];
+                    else r.w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(x)[e0 + e] << (16 * (e & 1));
+                }
+        }
     }
-    return r;
-}
+    __device__ __forceinline__ SqRaw<T, E> take(const T*, int, int, uintptr_t, uintptr_t) { return r; }
+};
+
+template <typename T, int E>
+struct SqLoad<T, kSqShifted, E> {
+    SqBytes<false> b;
+    __device__ __forceinline__ void issue(const T* x, int e0, int width, uintptr_t lo, uintptr_t hi) {
+        b.issue(reinterpret_cast<uintptr_t>(x + e0), reinterpret_cast<uintptr_t>(x + width), lo, hi);
+    }
+    __device__ __forceinline__ SqRaw<T, E> take(const T* x, int e0, int width, uintptr_t lo, uintptr_t hi) {
+        const uint4 v = b.take(reinterpret_cast<uintptr_t>(x + e0), reinterpret_cast<uintptr_t>(x + width), lo, hi);
+        SqRaw<T, E> r;
+        memcpy(r.w, &v, sizeof(r.w));
+        return r;
+    }
+};
 
 // |x| as fp32 bits from the bit pattern that SqRaw::top raised (halves joined).
 // The maximum is taken over bit patterns: there NaN > infinity > every number.
@@ -207,12 +331,20 @@ __device__ __forceinline__ void sq_codes(const SqRaw<T, E>& x, const SqScale& s,
 // stores the codes of values e0 .. e0 + E - 1 of a group of `width` values (e0 <
 // width) at cr (the group's first byte); values past the group's end are 0, so
 // the last odd value's byte has an empty high half
-template <typename T, int BITS, bool VEC, int E>
+template <typename T, int BITS, int MODE, int E>
 __device__ __forceinline__ void sq_store(uint8_t* cr, int e0, int width, const SqRaw<T, E>& x, const SqScale& s) {
     uint32_t q[(E * BITS + 31) / 32];
     sq_codes<T, BITS, E>(x, s, q);
     constexpr int W = E * BITS / 8;              // bytes of a chunk
     uint8_t* to = cr + e0 * BITS / 8;
+    if constexpr (MODE == kSqShifted) {
+        if (e0 + E > width) {
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                if (e0 + w * 8 / BITS < width) to[w] = (uint8_t)(q[w >> 2] >> (8 * (w & 3)));
+            return;
+        }
+    }
     if constexpr (W == 8) *reinterpret_cast<uint2*>(to) = make_uint2(q[0], q[1]);
     else if constexpr (W == 4) *reinterpret_cast<uint32_t*>(to) = q[0];
     else if constexpr (W == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)q[0];

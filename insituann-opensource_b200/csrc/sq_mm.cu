@@ -54,105 +54,16 @@ struct MmDot {
     int kp;                                     // bytes of a token's codes in shared memory
 };
 
-// 16 bytes of a row in flight: issue() starts the loads and has no branch, so
-// that several of them are under way at once; take() gives the bytes, with 0
-// past the row's end.  ALIGNED: rows are 16-byte aligned; else the two aligned
-// 16-byte pieces around the bytes are read and shifted.  A piece that is not
-// wholly inside the array [lo, hi) (at its ends only) is read by bytes.
-template <bool ALIGNED>
-struct MmBytes {
-    uint32_t v[ALIGNED ? 4 : 8];
-
-    // bytes [at, at + 16) of a row that ends at `end` (at >= end: none)
-    __device__ __forceinline__ void issue(uintptr_t at, uintptr_t end, uintptr_t lo, uintptr_t hi) {
-        if constexpr (ALIGNED) {
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (at + 16 <= end) x = __ldg(reinterpret_cast<const uint4*>(at));
-            v[0] = x.x;
-            v[1] = x.y;
-            v[2] = x.z;
-            v[3] = x.w;
-        } else {
-            const uintptr_t w = at & ~uintptr_t(15);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                if (at < end && w + 16 * h < end && w + 16 * h >= lo && w + 16 * h + 16 <= hi)
-                    x = __ldg(reinterpret_cast<const uint4*>(w + 16 * h));
-                v[4 * h] = x.x;
-                v[4 * h + 1] = x.y;
-                v[4 * h + 2] = x.z;
-                v[4 * h + 3] = x.w;
-            }
-        }
-    }
-    __device__ __forceinline__ uint4 take(uintptr_t at, uintptr_t end, uintptr_t lo, uintptr_t hi) {
-        if constexpr (ALIGNED) {
-            if (at < end && at + 16 > end) {                     // the last bytes of a row
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = edge(at + 4 * i, at, end);
-            }
-            return make_uint4(v[0], v[1], v[2], v[3]);
-        } else {
-            const uintptr_t w = at & ~uintptr_t(15);
-            if (at < end && (w < lo || w + 32 > hi)) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (w + (i & 4) * 4 < lo || w + (i & 4) * 4 + 16 > hi) v[i] = edge(w + 4 * i, lo, hi);
-            }
-            const uint4 x = shifted(at);
-            uint32_t o[4] = {x.x, x.y, x.z, x.w};
-            if (at + 16 > end) {                                 // clear what follows the row
-                const int left = at < end ? (int)(end - at) : 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int n = left - 4 * i;
-                    o[i] = n >= 4 ? o[i] : n <= 0 ? 0u : o[i] & ((1u << (8 * n)) - 1u);
-                }
-            }
-            return make_uint4(o[0], o[1], o[2], o[3]);
-        }
-    }
-    // the same where [at - 15, at + 32) is known to be inside the array and [at, at + 16) inside the row
-    __device__ __forceinline__ void issue_inside(uintptr_t at) {
-        const uint4* w = reinterpret_cast<const uint4*>(at & ~uintptr_t(15));
-        const uint4 x = __ldg(w), y = __ldg(w + 1);
-        v[0] = x.x;
-        v[1] = x.y;
-        v[2] = x.z;
-        v[3] = x.w;
-        v[4] = y.x;
-        v[5] = y.y;
-        v[6] = y.z;
-        v[7] = y.w;
-    }
-    // the 16 bytes from at & 15 on: by two words, by one, by bits
-    __device__ __forceinline__ uint4 shifted(uintptr_t at) {
-        const bool two = (at & 8) != 0, one = (at & 4) != 0;
-#pragma unroll
-        for (int i = 0; i < 6; ++i) v[i] = two ? v[i + 2] : v[i];
-#pragma unroll
-        for (int i = 0; i < 5; ++i) v[i] = one ? v[i + 1] : v[i];
-        const uint32_t sh = (uint32_t)(at & 3) * 8;
-        return make_uint4(__funnelshift_r(v[0], v[1], sh), __funnelshift_r(v[1], v[2], sh),
-                          __funnelshift_r(v[2], v[3], sh), __funnelshift_r(v[3], v[4], sh));
-    }
-    // the word at w, 0 where its bytes are outside [lo, hi)
-    static __device__ __forceinline__ uint32_t edge(uintptr_t w, uintptr_t lo, uintptr_t hi) {
-        uint32_t x = 0;
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i)
-            if (w + i >= lo && w + i < hi) x |= (uint32_t)*reinterpret_cast<const uint8_t*>(w + i) << (8 * i);
-        return x;
-    }
-};
-
 // quantises one floating row of k values into shared memory (one scale), by the whole block
-template <typename T, bool VEC>
+template <typename T, int MODE>
 __device__ __forceinline__ void dot_quantise(const T* x, int k, uint8_t* codes, float* scale, uint32_t* s_top) {
-    constexpr int E = sq_chunk<T, 8, VEC>();
+    constexpr int E = sq_chunk<T, 8, MODE>();
     uint32_t top = 0;
-    for (int e0 = threadIdx.x * E; e0 < k; e0 += kDotThreads * E) sq_load<T, VEC, E>(x, e0, k).top(top);
+    SqLoad<T, MODE, E> v;
+    for (int e0 = threadIdx.x * E; e0 < k; e0 += kDotThreads * E) {
+        v.issue(x, e0, k, 0, 0);
+        v.take(x, e0, k, 0, 0).top(top);
+    }
     top = __reduce_max_sync(0xffffffffu, __float_as_uint(sq_top<T>(top)));
     __syncthreads();
     if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
@@ -161,15 +72,17 @@ __device__ __forceinline__ void dot_quantise(const T* x, int k, uint8_t* codes, 
 #pragma unroll
     for (int w = 0; w < kDotThreads / 32; ++w) top = max(top, s_top[w]);
     const SqScale s = sq_scale<8>(__uint_as_float(top));
-    for (int e0 = threadIdx.x * E; e0 < k; e0 += kDotThreads * E)
-        sq_store<T, 8, VEC, E>(codes, e0, k, sq_load<T, VEC, E>(x, e0, k), s);
+    for (int e0 = threadIdx.x * E; e0 < k; e0 += kDotThreads * E) {
+        v.issue(x, e0, k, 0, 0);
+        sq_store<T, 8, MODE, E>(codes, e0, k, v.take(x, e0, k, 0, 0), s);
+    }
     if (threadIdx.x == 0) *scale = s.scale;
 }
 template <typename T>
 __device__ __forceinline__ void dot_quantise(const MmDot& q, int i, uint8_t* codes, float* scale, uint32_t* s_top) {
     const T* x = static_cast<const T*>(q.x) + i * q.ldx;
-    if (q.x_vec) dot_quantise<T, true>(x, q.p.k, codes, scale, s_top);
-    else dot_quantise<T, false>(x, q.p.k, codes, scale, s_top);
+    if (q.x_vec) dot_quantise<T, kSqVec>(x, q.p.k, codes, scale, s_top);
+    else dot_quantise<T, kSqSingle>(x, q.p.k, codes, scale, s_top);
 }
 
 // sums acc[0 .. N) over the 2 O lanes that differ in the bits below 2 O; the lane's
@@ -218,7 +131,7 @@ __global__ void __launch_bounds__(kDotThreads, kDotCtas<MT, R>) mm_dot_kernel(Mm
             const uintptr_t lo = reinterpret_cast<uintptr_t>(p.a), hi = lo + (m - 1) * p.lda + p.k;
             const uintptr_t a = lo + i * p.lda;
             for (int t = threadIdx.x; t < q.kp / 16; t += kDotThreads) {
-                MmBytes<false> w;
+                SqBytes<false> w;
                 w.issue(a + 16 * t, a + p.k, lo, hi);
                 reinterpret_cast<uint4*>(row)[t] = w.take(a + 16 * t, a + p.k, lo, hi);
             }
@@ -243,7 +156,7 @@ __global__ void __launch_bounds__(kDotThreads, kDotCtas<MT, R>) mm_dot_kernel(Mm
         for (int v = 0; v < V; ++v) acc[v] = 0;
 #pragma unroll R <= 2 ? 8 / R : 2
         for (int t = tl * 16; t < q.kp; t += TEAM * 16) {
-            MmBytes<ALIGNED> raw[R];
+            SqBytes<ALIGNED> raw[R];
 #pragma unroll
             for (int r = 0; r < R; ++r) raw[r].issue(b[r] + t, end[r], lo, hi);
             uint4 w[R];
@@ -293,12 +206,13 @@ cudaError_t go_dot(const MmDot& q, cudaStream_t st) {
     return cudaGetLastError();
 }
 
-// Rows of up to 128 bytes: 8 lanes a row, so that a warp reads 4 rows at once.
-// Longer ones take the warp; a single token takes fewer rows a warp where there
+// As many lanes a row as its 16-byte pieces need: 2, 8 or 16, else the warp; a single token takes fewer rows a warp where there
 // are few rows, so that all SMs have warps (1 x 4096 x 4096: 9.3 us with 4 rows, 7.3 us with 2).
 template <int MT, bool ALIGNED>
 cudaError_t by_team(const MmDot& q, cudaStream_t st) {
+    if (q.kp <= 32) return go_dot<MT, 2, 4, ALIGNED>(q, st);
     if (q.kp <= 128) return go_dot<MT, 8, MT == 1 ? 8 : 4, ALIGNED>(q, st);
+    if (q.kp <= 256) return go_dot<MT, 16, MT == 1 ? 8 : 4, ALIGNED>(q, st);
     if constexpr (MT == 1) {
         if (q.p.n < 4096) return go_dot<MT, 32, 1, ALIGNED>(q, st);
         if (q.p.n < 10000) return go_dot<MT, 32, 2, ALIGNED>(q, st);
@@ -308,7 +222,7 @@ cudaError_t by_team(const MmDot& q, cudaStream_t st) {
 
 // bytes of a token's codes that a team's lanes read: whole steps of the team
 int dot_kp(int k) {
-    const int step = k <= 128 ? 128 : 512;
+    const int step = k <= 32 ? 32 : k <= 128 ? 128 : k <= 256 ? 256 : 512;
     return (k + step - 1) / step * step;
 }
 
@@ -334,13 +248,10 @@ cudaError_t launch_dot(MmDot q, cudaStream_t st) {
 // A unit of work is a tile, or, with `split` > 1, one of the `split` parts of a
 // tile's k; a CTA takes the units blockIdx.x, + gridDim.x, ... (one unit each when
 // k is split):
-//   warp 0      (TMA) one lane issues the tensor copies, 128 bytes of k of the
-//               tile's rows of b and a per stage, 128-byte swizzled, through
-//               tensor maps over this GPU's memory (no multicast); rows and
-//               bytes past the ends read as zeros;
-//   last warps  (not TMA: rows that are not 16-byte aligned) kLoad warps put 16
-//               bytes together from aligned words and store them where the
-//               tensor copy would;
+//   warp 0      one lane issues the tensor copies, 128 bytes of k of the tile's
+//               rows of b and a per stage, 128-byte swizzled, through tensor
+//               maps over this GPU's memory (no multicast); rows and bytes past
+//               the ends read as zeros;
 //   warp 1      allocates tensor memory; one lane issues the MMAs (32 bytes of
 //               k each) into one of two accumulators of NT columns;
 //   warps 2..   epilogue: scales, bias, rounding and stores, while the next
@@ -353,13 +264,12 @@ cudaError_t launch_dot(MmDot q, cudaStream_t st) {
 constexpr int kMmM = 128, kMmK = 128;
 constexpr int kMmMaxStages = 12;
 
-template <int NT, bool TMA>
+template <int NT>
 struct MmCfg {
     static constexpr int kStage = (kMmM + NT) * kMmK;
-    static constexpr int kEpi = !TMA ? 4 : NT >= 256 ? 16 : NT >= 64 ? 8 : 4;   // epilogue warps
-    static constexpr int kLoad = TMA ? 0 : 16;                    // loading warps
-    static constexpr int kThreads = 64 + 32 * (kEpi + kLoad);
-    static constexpr int kCtas = TMA && NT <= 128 ? 2 : 1;        // resident per SM
+    static constexpr int kEpi = NT >= 256 ? 16 : NT >= 64 ? 8 : 4;   // epilogue warps
+    static constexpr int kThreads = 64 + 32 * kEpi;
+    static constexpr int kCtas = NT <= 128 ? 2 : 1;               // resident per SM
     static constexpr int kCols = 2 * NT;                          // tensor-memory columns
     static constexpr int kHalf = NT / (kEpi / 4);                 // columns of an epilogue warp
     static constexpr int kChunk = kHalf < 32 ? kHalf : 32;
@@ -447,6 +357,7 @@ struct MmTc {
     uint32_t tn, tm;            // channel and token tiles, fewer than 2^31 in all
     int split;                  // parts of k (the cluster's size)
     int kb_part;                // 128-byte blocks of k per part
+    uint32_t copy_bytes;        // of a stage's two tensor copies
     bool pair;                  // 2 neighbouring 16-bit outputs may be stored at once
 };
 
@@ -533,11 +444,11 @@ __device__ __forceinline__ void mm_block(const MmTc& q, int64_t at, const uint32
     else go(static_cast<__nv_bfloat16*>(q.p.out));
 }
 
-template <int NT, bool TMA>
-__global__ void __launch_bounds__(MmCfg<NT, TMA>::kThreads, MmCfg<NT, TMA>::kCtas)
+template <int NT>
+__global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
     mm_tc_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
                  const __grid_constant__ MmTc q) {
-    using C = MmCfg<NT, TMA>;
+    using C = MmCfg<NT>;
     extern __shared__ unsigned char sm_raw[];
     unsigned char* sm =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
@@ -565,7 +476,7 @@ __global__ void __launch_bounds__(MmCfg<NT, TMA>::kThreads, MmCfg<NT, TMA>::kCta
     }
     if (tid == 0) {
         for (int s = 0; s < C::kStages; ++s) {
-            mbar_init(&bar_full[s], TMA ? 1 : 4);                // the copying lane, or the warps of a loading group
+            mbar_init(&bar_full[s], 1);
             mbar_init(&bar_empty[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -581,7 +492,7 @@ __global__ void __launch_bounds__(MmCfg<NT, TMA>::kThreads, MmCfg<NT, TMA>::kCta
     const uint32_t tmem = s_tmem;
 
     if (warp == 0) {
-        if (TMA && lane == 0) {
+        if (lane == 0) {
             MmRing r;
             for (uint32_t t = t0; t < tiles && !*vfail; t += gridDim.x) {
                 int ct, tt;
@@ -592,7 +503,7 @@ __global__ void __launch_bounds__(MmCfg<NT, TMA>::kThreads, MmCfg<NT, TMA>::kCta
                         break;
                     }
                     unsigned char* st = sm + (size_t)r.s * C::kStage;
-                    mbar_arrive_expect(&bar_full[r.s], C::kStage);
+                    mbar_arrive_expect(&bar_full[r.s], q.copy_bytes);
                     tma_load_2d(st, &map_b, kb * kMmK, ct * kMmM, &bar_full[r.s]);
                     tma_load_2d(st + kMmM * kMmK, &map_a, kb * kMmK, tt * NT, &bar_full[r.s]);
                     r.next(C::kStages);
@@ -637,7 +548,7 @@ __global__ void __launch_bounds__(MmCfg<NT, TMA>::kThreads, MmCfg<NT, TMA>::kCta
             mm_drain(bar_empty, r, C::kStages);
         }
         __syncwarp();
-    } else if (warp < 2 + C::kEpi) {
+    } else {
         const int ew = warp - 2, quarter = warp & 3, side = ew >> 2;
         float* sc = s_scale[ew];
         uint32_t n = 0;                                          // tiles done
@@ -694,66 +605,6 @@ __global__ void __launch_bounds__(MmCfg<NT, TMA>::kThreads, MmCfg<NT, TMA>::kCta
                 __syncwarp();
                 mm_block(q, tok * p.ldo + ch, v, sc, cnt, sb, bias, (int)min((int64_t)32, p.n - (ch - lane)), lane);
                 __syncwarp();
-            }
-        }
-    } else if constexpr (!TMA) {
-        // Groups of 4 warps take the stages in turn, so that one group's loads, stores and fence overlap the
-        // others' (all 16 warps on every stage took twice as long).  A thread loads 16 bytes, chunk c, of the rows
-        // r0, r0 + 16, ..., four at a time.
-        constexpr int kGroups = C::kLoad / 4, kPer = (kMmM + NT) / 16;
-        static_assert(kPer % 4 == 0 && kMmM % 64 == 0, "four rows at a time are of one operand");
-        const int lt = tid - 64 - 32 * C::kEpi, r0 = (lt & 127) >> 3, c = lt & 7;
-        const uint32_t group = (uint32_t)lt >> 7;
-        const uintptr_t b_lo = reinterpret_cast<uintptr_t>(p.b), b_hi = b_lo + (p.n - 1) * p.ldb + p.k;
-        const uintptr_t a_lo = reinterpret_cast<uintptr_t>(p.a), a_hi = a_lo + (p.m - 1) * p.lda + p.k;
-        uint32_t i = 0;                                          // stages of all groups so far
-        bool ok = true;
-        for (uint32_t t = t0; ok && t < tiles; t += gridDim.x) {
-            int ct, tt;
-            mm_place(t, q.tn, q.tm, ct, tt);
-            for (int kb = kb0; kb < kb1; ++kb, ++i) {
-                if (i % kGroups != group) continue;
-                const uint32_t s = i % C::kStages, lap = i / C::kStages;
-                if (lap > 0) ok = __all_sync(0xffffffffu, mm_wait(&bar_empty[s], (lap - 1) & 1, vfail));
-                if (!ok) {
-                    if (lane == 0) s_fail = 1;
-                    break;
-                }
-                unsigned char* st = sm + (size_t)s * C::kStage + r0 * 128 + ((c ^ (r0 & 7)) << 4);
-                // no load of this step leaves its row by more than the 16-byte pieces around it, nor the arrays
-                const bool inner = (kb + 1) * kMmK + 16 <= p.k && ((a_lo | b_lo) & 15) == 0;
-#pragma unroll 1
-                for (int u0 = 0; u0 < kPer; u0 += 4) {
-                    const bool is_b = u0 * 16 < kMmM;
-                    const uintptr_t lo = is_b ? b_lo : a_lo, hi = is_b ? b_hi : a_hi;
-                    const int64_t ld = is_b ? p.ldb : p.lda, rows = is_b ? p.n : p.m;
-                    const int64_t row = (is_b ? (int64_t)ct * kMmM : (int64_t)tt * NT - kMmM) + r0 + u0 * 16;
-                    MmBytes<false> raw[4];
-                    uintptr_t at[4], end[4];                     // a row past the last one is empty
-                    if (inner && row - r0 + 64 <= rows) {
-                        const uintptr_t first = lo + row * ld + kb * kMmK + 16 * c;
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) raw[u].issue_inside(first + u * 16 * ld);
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            *reinterpret_cast<uint4*>(st + (u0 + u) * 16 * 128) = raw[u].shifted(first + u * 16 * ld);
-                        continue;
-                    }
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const bool in = row + u * 16 < rows;
-                        const uintptr_t first = lo + (in ? row + u * 16 : 0) * ld;
-                        at[u] = first + kb * kMmK + 16 * c;
-                        end[u] = in ? first + p.k : 0;
-                        raw[u].issue(at[u], end[u], lo, hi);
-                    }
-#pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        *reinterpret_cast<uint4*>(st + (u0 + u) * 16 * 128) = raw[u].take(at[u], end[u], lo, hi);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar_full[s]);
             }
         }
     }
@@ -824,28 +675,29 @@ cudaError_t mm_map_rows(const int8_t* rows, int64_t n, int k, int64_t ld, int bo
 // whether 2 neighbouring 16-bit outputs of a row may be stored at once
 bool pair_out(const SqMatmul& p, int out_type) { return out_type != kSqF32 && rows_aligned(p.out, 2 * p.ldo, 4); }
 
-template <int NT, bool TMA>
+template <int NT>
 cudaError_t go_tc(const SqMatmul& p, int out_type, int split, cudaStream_t st) {
-    using C = MmCfg<NT, TMA>;
+    using C = MmCfg<NT>;
     CUtensorMap map_b{}, map_a{};
-    cudaError_t e = cudaSuccess;
-    if (TMA) {
-        e = mm_map_rows(p.b, p.n, p.k, p.ldb, kMmM, &map_b);
-        if (!e) e = mm_map_rows(p.a, p.m, p.k, p.lda, NT, &map_a);
-    }
-    if (!e) e = cudaFuncSetAttribute(mm_tc_kernel<NT, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
+    // A box has no more rows than its operand: filling in those that are not there took longer than copying rows
+    // (2693 x 11 x 4836: 1.6 us a step of k).  What the shared memory holds in their place only
+    // reaches accumulators of channels and tokens that are not there either.
+    const int box_b = (int)std::min<int64_t>(kMmM, p.n), box_a = (int)std::min<int64_t>(NT, p.m);
+    cudaError_t e = mm_map_rows(p.b, p.n, p.k, p.ldb, box_b, &map_b);
+    if (!e) e = mm_map_rows(p.a, p.m, p.k, p.lda, box_a, &map_a);
+    if (!e) e = cudaFuncSetAttribute(mm_tc_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
     if (e) return e;
     MmTc q{};
     q.p = p;
     q.out_type = out_type;
     q.pair = pair_out(p, out_type);
+    q.copy_bytes = (uint32_t)(box_a + box_b) * kMmK;
     q.tn = (uint32_t)((p.n + kMmM - 1) / kMmM);
     q.tm = (uint32_t)((p.m + NT - 1) / NT);
     if ((int64_t)q.tn * q.tm >= int64_t(1) << 31) return cudaErrorInvalidValue;
     const int kb = (p.k + kMmK - 1) / kMmK;
     q.kb_part = (kb + split - 1) / split;
-    q.split = (kb + q.kb_part - 1) / q.kb_part == split ? split : 1;     // every part has work
-    if (q.split == 1) q.kb_part = kb;
+    q.split = (kb + q.kb_part - 1) / q.kb_part;                  // every part has work
     const int64_t tiles = (int64_t)q.tn * q.tm;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(q.split > 1 ? tiles * q.split : std::min<int64_t>(tiles, (int64_t)sm_count() * C::kCtas)));
@@ -859,14 +711,14 @@ cudaError_t go_tc(const SqMatmul& p, int out_type, int split, cudaStream_t st) {
     cfg.attrs = at;
     cfg.numAttrs = 1;
     note_launch();
-    return cudaLaunchKernelEx(&cfg, mm_tc_kernel<NT, TMA>, map_b, map_a, q);
+    return cudaLaunchKernelEx(&cfg, mm_tc_kernel<NT>, map_b, map_a, q);
 }
 
 // Which tile and how many parts of k: the least of an estimate, in us, that was
 // fitted to sweeps of 30 shapes from 16 x 512 x 8192 to 256 x 1M x 128 on a B200
 // (the choice is within 10 % of the best of each sweep).  An SM draws what it
-// has in flight per 1.6 us of latency under load, whole stages of its resident
-// CTAs; b comes from HBM at 5 TB/s or from L2; a unit's epilogue costs 0.35 us
+// has in flight per 1.6 us of latency under load, the stages of its resident
+// CTAs, at most 130 bytes a ns; b comes from HBM at 5 TB/s or from L2; a unit's epilogue costs 0.35 us
 // and 1 us per 13000 outputs; a split costs a cluster launch, two cluster barriers and the
 // sums' way through shared memory, and CTAs beyond those that are resident start anew.
 // With few tiles a split is worth much: 64 x 256 x 16384 takes 11.3 us in 8
@@ -876,20 +728,20 @@ struct MmPick {
     double us;
 };
 
-template <int NT, bool TMA>
+template <int NT>
 void mm_estimate(const SqMatmul& p, int sms, MmPick& best) {
-    using C = MmCfg<NT, TMA>;
-    if (NT > (TMA ? 16 : 64) && NT / 2 >= p.m) return;           // a smaller tile holds all tokens
+    using C = MmCfg<NT>;
+    if (NT > 16 && NT / 2 >= p.m) return;                        // a smaller tile holds all tokens
     const double tm = (double)((p.m + NT - 1) / NT), tiles = (double)((p.n + kMmM - 1) / kMmM) * tm;
     const int kb = (p.k + kMmK - 1) / kMmK;
-    const double rows = kMmM + std::min<int64_t>(NT, p.m), epi = 0.35 + NT * kMmM / 13000.0;
+    const double rows = std::min<int64_t>(kMmM, p.n) + std::min<int64_t>(NT, p.m), epi = 0.35 + NT * kMmM / 13000.0;
     for (int split = 1; split <= 8; split *= 2) {
         if (split > 1 && (kb < 2 * split || tiles * split > 8.0 * sms)) break;
-        const double per_sm = std::ceil(tiles * split / sms);
-        const double flight = std::min<double>(C::kCtas, per_sm) * C::kStage * C::kStages;
-        const double rate = TMA ? flight / 1.6e3 : 25.0;         // bytes a ns
-        const double part = (kb + split - 1) / split * (double)kMmK;
-        double us = std::max(per_sm * rows * part / rate / 1e3, (double)p.n * p.k / 5e6);
+        const double per_sm = std::ceil(tiles * split / sms), ctas = std::min<double>(C::kCtas, per_sm);
+        const int kb_part = (kb + split - 1) / split;
+        const double bytes = per_sm * kb_part * rows * kMmK;
+        double us = std::max(per_sm * kb_part * 1.6 / (C::kStages * ctas), bytes / 130e3);
+        us = std::max(us, (double)p.n * p.k / 5e6);
         us = 4.0 + std::max(us, per_sm * epi) + epi;
         if (split > 1) us += 1.6 + 0.01 * NT + 3.0 * (std::ceil(tiles * split / (sms * C::kCtas)) - 1);
         us *= 1.0 + 0.05 * std::min<double>(4.0, tm - 1.0);      // every token tile reads b again
@@ -900,49 +752,108 @@ void mm_estimate(const SqMatmul& p, int sms, MmPick& best) {
 cudaError_t launch_tc(const SqMatmul& p, int out_type, cudaStream_t st) {
     MmPick pick{0, 1, 1e300};
     const int sms = sm_count();
-    if (!rows_aligned(p.a, p.lda, 16) || !rows_aligned(p.b, p.ldb, 16)) {
-        mm_estimate<64, false>(p, sms, pick);
-        mm_estimate<128, false>(p, sms, pick);
-        return pick.nt == 64 ? go_tc<64, false>(p, out_type, pick.split, st)
-                             : go_tc<128, false>(p, out_type, pick.split, st);
-    }
-    mm_estimate<16, true>(p, sms, pick);
-    mm_estimate<32, true>(p, sms, pick);
-    mm_estimate<64, true>(p, sms, pick);
-    mm_estimate<128, true>(p, sms, pick);
-    mm_estimate<256, true>(p, sms, pick);
+    mm_estimate<16>(p, sms, pick);
+    mm_estimate<32>(p, sms, pick);
+    mm_estimate<64>(p, sms, pick);
+    mm_estimate<128>(p, sms, pick);
+    mm_estimate<256>(p, sms, pick);
     switch (pick.nt) {
-        case 16: return go_tc<16, true>(p, out_type, pick.split, st);
-        case 32: return go_tc<32, true>(p, out_type, pick.split, st);
-        case 64: return go_tc<64, true>(p, out_type, pick.split, st);
-        case 128: return go_tc<128, true>(p, out_type, pick.split, st);
-        default: return go_tc<256, true>(p, out_type, pick.split, st);
+        case 16: return go_tc<16>(p, out_type, pick.split, st);
+        case 32: return go_tc<32>(p, out_type, pick.split, st);
+        case 64: return go_tc<64>(p, out_type, pick.split, st);
+        case 128: return go_tc<128>(p, out_type, pick.split, st);
+        default: return go_tc<256>(p, out_type, pick.split, st);
     }
+}
+
+// one token, or a few whose rows would have to be copied first: dot products
+bool use_dot(const SqMatmul& p, bool aligned) { return dot_usable(p) && (p.m == 1 || !aligned); }
+
+// ---- rows that are not 16-byte aligned -------------------------------------
+// The tensor copies need aligned rows; others are copied to scratch whose rows
+// are, 16 bytes a thread.  Putting the rows together inside the product, by
+// warps in the tensor copies' place, took longer (333 x 10007 x 1031: 37 us;
+// 5000^3: 490 us).
+int64_t mm_ld(int k) { return (k + 15) / 16 * 16; }
+
+__global__ void __launch_bounds__(256) mm_align_kernel(const int8_t* rows, int64_t n, int k, int64_t ld, int8_t* to,
+                                                       int64_t ldt) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(rows), hi = lo + (n - 1) * ld + k;
+    const int chunks = (int)(ldt / 16);
+    const uint64_t items = (uint64_t)n * chunks, step = (uint64_t)gridDim.x * 256 * 4;
+    for (uint64_t i0 = (uint64_t)blockIdx.x * 256 * 4 + threadIdx.x; i0 < items; i0 += step) {
+        SqBytes<false> raw[4];
+        uintptr_t at[4], end[4];
+        int8_t* out[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            uint32_t row = 0;
+            int c = 0;
+            const bool in = i0 + u * 256 < items;
+            sq_split(in ? i0 + u * 256 : 0, chunks, row, c);
+            const uintptr_t first = lo + (int64_t)row * ld;
+            at[u] = first + 16 * c;
+            end[u] = in ? first + k : 0;
+            out[u] = in ? to + (int64_t)row * ldt + 16 * c : nullptr;
+            raw[u].issue(at[u], end[u], lo, hi);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (out[u]) *reinterpret_cast<uint4*>(out[u]) = raw[u].take(at[u], end[u], lo, hi);
+    }
+}
+
+cudaError_t launch_align(const int8_t* rows, int64_t n, int k, int64_t ld, int8_t* to, cudaStream_t st) {
+    const int64_t items = n * (mm_ld(k) / 16), per = 256 * 4;
+    note_launch();
+    mm_align_kernel<<<(int)std::min<int64_t>((items + per - 1) / per, (int64_t)sm_count() * 16), 256, 0, st>>>(
+        rows, n, k, ld, to, mm_ld(k));
+    return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t sq_matmul(const SqMatmul& p, int out_type, cudaStream_t st) {
+size_t sq_matmul_work(const SqMatmul& p) {
+    if (p.m == 0 || p.n == 0) return 0;
+    const bool al_a = rows_aligned(p.a, p.lda, 16), al_b = rows_aligned(p.b, p.ldb, 16);
+    if (use_dot(p, al_a && al_b)) return 0;
+    return (size_t)mm_ld(p.k) * ((al_a ? 0 : (size_t)p.m) + (al_b ? 0 : (size_t)p.n));
+}
+
+cudaError_t sq_matmul(SqMatmul p, int out_type, void* work, cudaStream_t st) {
     if (p.m == 0 || p.n == 0) return cudaSuccess;
-    // one token, or a few where the tensor-core kernel would have to put its rows together: dot products
-    const bool aligned = rows_aligned(p.a, p.lda, 16) && rows_aligned(p.b, p.ldb, 16);
-    if (dot_usable(p) && (p.m == 1 || !aligned)) {
+    const bool al_a = rows_aligned(p.a, p.lda, 16), al_b = rows_aligned(p.b, p.ldb, 16);
+    if (use_dot(p, al_a && al_b)) {
         MmDot q{};
         q.p = p;
         q.out_type = out_type;
         return launch_dot(q, st);
     }
-    return launch_tc(p, out_type, st);
+    int8_t* to = static_cast<int8_t*>(work);
+    cudaError_t e = cudaSuccess;
+    if (!al_b) {
+        e = launch_align(p.b, p.n, p.k, p.ldb, to, st);
+        p.b = to;
+        p.ldb = mm_ld(p.k);
+        to += p.n * p.ldb;
+    }
+    if (!e && !al_a) {
+        e = launch_align(p.a, p.m, p.k, p.lda, to, st);
+        p.a = to;
+        p.lda = mm_ld(p.k);
+    }
+    return e ? e : launch_tc(p, out_type, st);
 }
 
-bool sq_scores_fused(int64_t m, int k) {
-    SqMatmul p{};
-    p.m = m;
-    p.k = k;
-    return dot_usable(p);
+size_t sq_scores_work(const SqMatmul& q) {
+    if (q.m == 0 || q.n == 0 || dot_usable(q)) return 0;
+    SqMatmul p = q;
+    p.a = nullptr;                                               // the tokens' codes are aligned
+    p.lda = mm_ld(p.k);
+    return (size_t)p.m * (size_t)(p.lda + 4) + 12 + sq_matmul_work(p);
 }
 
-cudaError_t sq_scores(const SqWrite& w, int x_type, SqMatmul p, int out_type, cudaStream_t st) {
+cudaError_t sq_scores(SqWrite w, int x_type, SqMatmul p, int out_type, void* work, cudaStream_t st) {
     if (p.m == 0 || p.n == 0) return cudaSuccess;
     if (dot_usable(p)) {
         MmDot q{};
@@ -955,12 +866,18 @@ cudaError_t sq_scores(const SqWrite& w, int x_type, SqMatmul p, int out_type, cu
         q.x_vec = rows_aligned(w.x, (int64_t)w.ldx * es, 16) && (p.k * es) % 16 == 0;
         return launch_dot(q, st);
     }
+    // work: the tokens' codes, their scales, then what the product needs
+    w.codes = static_cast<uint8_t*>(work);
+    w.ldc = (uint32_t)mm_ld(p.k);
+    w.scales = reinterpret_cast<float*>(w.codes + (size_t)p.m * w.ldc);
+    w.lds = 1;
+    w.capacity = w.n;
     const cudaError_t e = sq_write(w, x_type, 8, st);
     if (e) return e;
     p.a = reinterpret_cast<const int8_t*>(w.codes);
     p.a_scale = w.scales;
     p.lda = w.ldc;
-    return sq_matmul(p, out_type, st);
+    return sq_matmul(p, out_type, w.codes + ((size_t)p.m * (size_t)(w.ldc + 4) + 15) / 16 * 16, st);
 }
 
 }  // namespace isb

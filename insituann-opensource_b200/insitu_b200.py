@@ -45,7 +45,8 @@ EXPORTS = [
     "ivf_last_error", "ivf_global_last_error",
     "ivf_kernel_launches", "ivf_batch_profile", "ivf_batch_stage_ms", "ivf_u8_search_noalloc",
     "ivf_load_centroids", "ivf_assign", "ivf_build_reorder", "ivf_kmeans_update", "ivf_pq_train", "ivf_pq_encode",
-    "ivf_sq_write", "ivf_sq_read", "ivf_sq_matmul", "ivf_sq_scores", "ivf_sq_scores_work",
+    "ivf_sq_write", "ivf_sq_read", "ivf_sq_matmul", "ivf_sq_matmul_work", "ivf_sq_scores",
+    "ivf_sq_scores_work",
     "ivf_read_centroids", "ivf_read_assign", "ivf_read_codebook", "ivf_read_codes", "ivf_read_u8bin",
     "ivf_read_fbin", "ivf_read_gt", "ivf_write_centroids", "ivf_write_assign", "ivf_write_codebook",
     "ivf_write_codes", "ivf_pq_load_files", "ivf_pq_insert",
@@ -121,9 +122,10 @@ _SIGS = {
     "ivf_pq_encode": ([vp, i32, i64, i32, vp, vp, vp, vp, i32, vp, vp], i32),
     "ivf_sq_write": ([vp, i32, i64, i32, i64, vp, i32, i32, vp, i64, vp, i64, i64, vp, vp], i32),
     "ivf_sq_read": ([vp, i64, vp, i64, i64, i32, i32, vp, i64, i32, vp, i32, i64, vp], i32),
-    "ivf_sq_matmul": ([vp, i64, vp, i64, vp, i64, vp, i64, i32, vp, vp, i32, i64, vp], i32),
+    "ivf_sq_matmul": ([vp, i64, vp, i64, vp, i64, vp, i64, i32, vp, vp, i32, i64, vp, C.c_size_t, vp], i32),
+    "ivf_sq_matmul_work": ([vp, i64, i64, vp, i64, i64, i32], C.c_size_t),
     "ivf_sq_scores": ([vp, i32, i64, i64, vp, i64, vp, i64, i32, vp, vp, i32, i64, vp, C.c_size_t, vp], i32),
-    "ivf_sq_scores_work": ([i64, i32], C.c_size_t),
+    "ivf_sq_scores_work": ([i64, vp, i64, i64, i32], C.c_size_t),
     "ivf_read_centroids": ([C.c_char_p, vp, i64, vp, vp], i64),
     "ivf_read_assign": ([C.c_char_p, vp, i64, vp], i64),
     "ivf_read_codebook": ([C.c_char_p, vp, i64, vp, vp, vp], i64),
@@ -766,8 +768,13 @@ def sq_matmul(a, a_scale, b, b_scale, bias=None, dtype=None, out=None):
     dtype = dtype or (torch.float32 if out is None else out.dtype)
     t = _sq_type(dtype)
     out, ldo = _sq_out(out, m, n, dtype, dev)
-    _sq_call(L.ivf_sq_matmul, dev, a.data_ptr(), lda, a_scale.data_ptr(), m, b.data_ptr(), ldb, b_scale.data_ptr(),
-             n, k, None if bias is None else bias.data_ptr(), out.data_ptr(), t, ldo)
+    pa, pb, need, work = a.data_ptr(), b.data_ptr(), 0, None
+    if (pa | pb | lda | ldb) & 15:                       # rows that the library may have to copy first
+        need = L.ivf_sq_matmul_work(pa, lda, m, pb, ldb, n, k)
+        work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _sq_call(L.ivf_sq_matmul, dev, pa, lda, a_scale.data_ptr(), m, pb, ldb, b_scale.data_ptr(), n, k,
+             None if bias is None else bias.data_ptr(), out.data_ptr(), t, ldo,
+             None if work is None else work.data_ptr(), need)
     return out
 
 
@@ -907,7 +914,7 @@ class SQRows:
         dtype = dtype or (torch.float32 if out is None else out.dtype)
         to = _sq_type(dtype)
         out, ldo = _sq_out(out, m, self.capacity, dtype, self.device)
-        need = self.L.ivf_sq_scores_work(m, self.d)
+        need = self.L.ivf_sq_scores_work(m, self._codes.data_ptr(), self._ldc, self.capacity, self.d)
         work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         _sq_call(self.L.ivf_sq_scores, self.device, x.data_ptr(), t, ldx, m, self._codes.data_ptr(), self._ldc,
                  self._scales.data_ptr(), self.capacity, self.d, None if bias is None else bias.data_ptr(), out.data_ptr(),

@@ -332,6 +332,19 @@ def test_scores(cuda_ok, m, n, d, t):
         assert torch.equal(got, store.scores(wide[:, 1:1 + d], dtype=o, bias=bias))
 
 
+@pytest.mark.parametrize("m", [1, 3, 9, 40, 300])
+@pytest.mark.parametrize("d,pad,offset", [(100, 1, 0), (128, 0, 5), (33, 0, 8)])
+def test_scores_of_an_unaligned_store(cuda_ok, m, d, pad, offset):
+    n = 259
+    rows, _ = new_store(n, d, 8, 0, pad, offset)
+    x = rows_of(n, d, torch.float32, 4)
+    ref = ib.SQRows(n, d).write(x)
+    rows.write(x)
+    q = rows_of(m, d, torch.bfloat16, 5)
+    assert torch.equal(rows.scores(q), ref.scores(q))
+    assert torch.equal(rows.scores(q, dtype=torch.float16), ref.scores(q, dtype=torch.float16))
+
+
 def test_run_together(cuda_ok):
     """rows inserted, replaced, scored and read back: the best rows are the true neighbours, and rescoring the
     candidates with their values ranks them as the scores do"""

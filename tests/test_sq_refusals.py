@@ -18,7 +18,7 @@ WRITE = dict(x=P, x_type=0, n=4, d=32, ldx=32, slots=P, bits=8, group=0, codes=P
 READ = dict(codes=P, ldc=32, scales=P, lds=1, capacity=16, bits=8, group=0, slots=P, n=4, d=32, out=P, out_type=0,
             ldo=32, stream=None)
 MATMUL = dict(a=P, lda=32, a_scale=P, m=4, b=P, ldb=32, b_scale=P, n=8, k=32, bias=None, out=P, out_type=0, ldo=8,
-              stream=None)
+              work=None, work_bytes=0, stream=None)
 SCORES = dict(x=P, x_type=0, ldx=32, m=8, codes=P, ldc=32, scales=P, n=8, d=32, bias=None, out=P, out_type=0, ldo=8,
               work=P, work_bytes=1 << 20, stream=None)
 
@@ -53,7 +53,8 @@ def test_read_refuses(change):
     dict(m=-1), dict(m=1 << 31), dict(n=-1), dict(n=1 << 31), dict(k=0), dict(k=131072), dict(lda=31), dict(ldb=31),
     dict(ldo=7), dict(a=None), dict(b=None), dict(a_scale=None), dict(b_scale=None), dict(out=None),
     dict(out_type=7), dict(out=P + 2), dict(out_type=2, out=P + 1), dict(a_scale=P + 1), dict(b_scale=P + 2),
-    dict(bias=P + 3)])
+    dict(bias=P + 3), dict(work=P + 8), dict(m=8, a=P + 1), dict(m=8, b=P + 4, work=P, work_bytes=8 * 32 - 1),
+    dict(m=8, k=31, lda=31, work=P, work_bytes=8 * 32 - 1)])
 def test_matmul_refuses(change):
     rc, msg = call("ivf_sq_matmul", MATMUL, **change)
     assert rc == EINVAL and msg
@@ -78,13 +79,25 @@ def test_calls_without_rows_do_nothing():
     assert call("ivf_sq_scores", SCORES, n=0, codes=None, scales=None, out=None)[0] == OK
 
 
-def test_scores_work():
+def test_scratch_sizes():
     L = lib()
-    assert L.ivf_sq_scores_work(10, 96) >= 10 * (96 + 4)
-    assert L.ivf_sq_scores_work(10, 97) >= 10 * (112 + 4)
-    assert L.ivf_sq_scores_work((1 << 31) - 2, 131071) >= ((1 << 31) - 2) * (131072 + 4)
-    assert L.ivf_sq_scores_work(-1, 8) == L.ivf_sq_scores_work(8, 0) == L.ivf_sq_scores_work(8, 131072) == 0
-    assert L.ivf_sq_scores_work(1, 96) == L.ivf_sq_scores_work(0, 96) == 0     # nothing to keep between two kernels
+
+    def scores(m, d, codes=P, ldc=None, n=50):
+        return L.ivf_sq_scores_work(m, codes, ldc or (d + 15) // 16 * 16, n, d)
+
+    matmul = L.ivf_sq_matmul_work
+    assert scores(10, 96) >= 10 * (96 + 4)
+    assert scores(10, 97) >= 10 * (112 + 4)
+    assert scores(10, 96, codes=P + 1) >= 10 * (96 + 4) + 50 * 96          # a store whose rows are copied first
+    assert scores(10, 97, ldc=97) >= 10 * (112 + 4) + 50 * 112
+    assert scores((1 << 31) - 2, 131071) >= ((1 << 31) - 2) * (131072 + 4)
+    assert scores(1, 96) == scores(0, 96) == scores(10, 96, n=0) == 0      # nothing to keep between two kernels
+    assert scores(-1, 8) == scores(8, 0) == scores(8, 131072) == scores(10, 96, ldc=95) == 0
+    assert matmul(P, 48, 10, P, 64, 20, 33) == 0
+    assert matmul(P + 1, 48, 10, P, 64, 20, 33) == 10 * 48
+    assert matmul(P, 48, 10, P, 33, 20, 33) == 20 * 48
+    assert matmul(P, 33, 10, P, 33, 20, 33) == 30 * 48
+    assert matmul(P, 33, 1, P, 33, 20, 33) == matmul(P, 33, 0, P, 33, 20, 33) == matmul(P, 32, 10, P, 33, 20, 33) == 0
 
 
 def test_binding_refuses_without_a_device():
