@@ -251,7 +251,8 @@ struct SqRead {
     uint32_t n, ldo;
     int d;
     void* out;                   // [n, d], ldo values apart
-    bool once;                   // set by sq_read
+    bool once;                   // set by sq_read, as is
+    int group_log;               // log2 of group, -1 where it is no power of two
 };
 cudaError_t sq_read(SqRead p, int type, int bits, cudaStream_t st);
 struct SqMatmul {

@@ -81,10 +81,9 @@ __global__ void __launch_bounds__(kSqThreads, CH > 4 ? 2 : MODE == kSqShifted &&
 // One block per group, for groups that do not fit a warp's registers: a thread
 // keeps its first CH chunks; what a group has beyond kSqThreads * CH is read
 // again, from the caches.
-template <typename T, int BITS, int MODE>
-__global__ void __launch_bounds__(kSqThreads) sq_write_long_kernel(SqWrite p) {
+template <typename T, int BITS, int MODE, int CH>
+__global__ void __launch_bounds__(kSqThreads, CH <= 2 ? 4 : MODE == kSqShifted ? 1 : 3) sq_write_long_kernel(SqWrite p) {
     constexpr int E = sq_chunk<T, BITS, MODE>();
-    constexpr int CH = 8;
     __shared__ uint32_t s_top[kSqThreads / 32];
     const uintptr_t lo = reinterpret_cast<uintptr_t>(p.x), hi = lo + ((uint64_t)(p.n - 1) * p.ldx + p.d) * sizeof(T);
     const uint64_t items = (uint64_t)p.n * (uint32_t)p.groups;
@@ -206,7 +205,8 @@ cudaError_t launch_write(const SqWrite& p, cudaStream_t st) {
     }
     const int grid = (int)std::min<int64_t>((int64_t)p.n * p.groups, (int64_t)sm_count() * 8);
     note_launch();
-    sq_write_long_kernel<T, BITS, MODE><<<grid, kSqThreads, 0, st>>>(p);
+    if (chunks <= 2 * kSqThreads) sq_write_long_kernel<T, BITS, MODE, 2><<<grid, kSqThreads, 0, st>>>(p);
+    else sq_write_long_kernel<T, BITS, MODE, 8><<<grid, kSqThreads, 0, st>>>(p);
     return cudaGetLastError();
 }
 
