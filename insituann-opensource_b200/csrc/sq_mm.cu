@@ -206,8 +206,9 @@ cudaError_t go_dot(const MmDot& q, cudaStream_t st) {
     return cudaGetLastError();
 }
 
-// As many lanes a row as its 16-byte pieces need: 2, 8 or 16, else the warp; a single token takes fewer rows a warp where there
-// are few rows, so that all SMs have warps (1 x 4096 x 4096: 9.3 us with 4 rows, 7.3 us with 2).
+// As many lanes a row as its 16-byte pieces need: 2, 8 or 16, else the warp.  A
+// single token takes fewer rows a warp where there are few rows, so that all
+// SMs have warps (1 x 4096 x 4096: 9.3 us with 4 rows, 7.3 us with 2).
 template <int MT, bool ALIGNED>
 cudaError_t by_team(const MmDot& q, cudaStream_t st) {
     if (q.kp <= 32) return go_dot<MT, 2, 4, ALIGNED>(q, st);
@@ -273,8 +274,8 @@ struct MmCfg {
     static constexpr int kCols = 2 * NT;                          // tensor-memory columns
     static constexpr int kHalf = NT / (kEpi / 4);                 // columns of an epilogue warp
     static constexpr int kChunk = kHalf < 32 ? kHalf : 32;
-    static constexpr int kStatic = kEpi * kChunk * 4 + 1024;   // static arrays and the system's 1 KB
-    static constexpr int kFit = (227 * 1024 / kCtas - 1024 - 1024 - kStatic) / kStage;
+    static constexpr int kStatic = kEpi * kChunk * 4 + 1024;      // static arrays
+    static constexpr int kFit = (227 * 1024 / kCtas - 1024 - 1024 - kStatic) / kStage;   // 1 KB to align, 1 KB of the system's
     static constexpr int kStages = kFit < kMmMaxStages ? kFit : kMmMaxStages;
     static constexpr size_t kSmem = (size_t)kStage * kStages + 1024;
     static_assert(kStages >= 2 && (size_t)kMmM * NT * 4 <= (size_t)kStage * kStages, "a split tile's sums fit the stages");
@@ -296,8 +297,8 @@ __device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, const vo
 }
 
 // The copying and the MMA thread run once per 128 bytes of k, some 500 clocks of
-// the tensor core: their place in the ring of stages is counted, not divided out (a 64-bit
-// remainder a step cost a fifth of the rate).
+// the tensor core: their place in the ring of stages is counted, not divided
+// out (a 64-bit remainder a step made 8192^3 a tenth slower).
 struct MmRing {
     uint32_t s = 0, lap = 0;                    // stage, times round the ring
     __device__ __forceinline__ void next(uint32_t stages) {
@@ -367,10 +368,11 @@ struct MmTc {
 // With output-bound products (k near 128) the instructions of this loop decide.
 // Two tokens are scaled at once by packed fp32 pairs; sums of at most 2^22
 // (SMALL: k <= 256) become floats by adding 1.5 * 2^23 as bits, which is exact
-// and leaves the slow integer conversion out; and 16-bit outputs (PAIR: rows
+// and leaves the slow integer conversion out; and 16-bit outputs (pair: rows
 // 4-byte aligned) are exchanged with the neighbouring lane, so that each lane
-// stores 2 channels of one token.  Turning the block in shared memory for 16-byte stores was slower (fp32
-// scores of 256 x 1M: 283 against 222 us): its round trips wait longer than the stores saved.
+// stores 2 channels of one token.  Turning the block in shared memory for
+// 16-byte stores was slower (fp32 scores of 256 x 1M: 283 against 222 us): its
+// round trips wait longer than the stores they save.
 template <bool SMALL>
 __device__ __forceinline__ float2 mm_scaled(uint32_t v0, uint32_t v1, float2 sa, float sb, float bias) {
     constexpr float kMagic = 12582912.f;
@@ -517,7 +519,7 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
         if (lane == 0) {
             constexpr uint32_t idesc = umma_idesc_s8(kMmM, NT);
             const uint64_t desc0 = umma_smem_desc_sw128(smem_u32(sm));
-            const int last = (p.k - (kb1 - 1) * kMmK + 31) / 32;          // MMAs of the last step of k (1 to 4 are needed)
+            const int last = (p.k - (kb1 - 1) * kMmK + 31) / 32;          // MMAs of the last step of k, at least
             MmRing r;
             uint32_t n = 0;                                      // tiles done
             for (uint32_t t = t0; t < tiles; t += gridDim.x, ++n) {
@@ -574,7 +576,8 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
             if (!ok && lane == 0) s_fail = 1;
             tc_fence_after();
             if (split > 1) {
-                // this part's sums to shared memory (the stages are read: the accumulator is done), [column][channel]
+                // this part's sums to shared memory, [column][channel] (the stages
+                // are read: the accumulator is done)
                 int* x = reinterpret_cast<int*>(sm) + (size_t)side * C::kHalf * kMmM + quarter * 32 + lane;
                 for (int c = 0; c < C::kHalf; c += C::kChunk) {
                     uint32_t v[C::kChunk];
@@ -679,9 +682,9 @@ template <int NT>
 cudaError_t go_tc(const SqMatmul& p, int out_type, int split, cudaStream_t st) {
     using C = MmCfg<NT>;
     CUtensorMap map_b{}, map_a{};
-    // A box has no more rows than its operand: filling in those that are not there took longer than copying rows
-    // (2693 x 11 x 4836: 1.6 us a step of k).  What the shared memory holds in their place only
-    // reaches accumulators of channels and tokens that are not there either.
+    // A box has no more rows than its operand: rows that are not there take
+    // time to fill in.  What the shared memory holds in their place only reaches
+    // accumulators of channels and tokens that are not there either.
     const int box_b = (int)std::min<int64_t>(kMmM, p.n), box_a = (int)std::min<int64_t>(NT, p.m);
     cudaError_t e = mm_map_rows(p.b, p.n, p.k, p.ldb, box_b, &map_b);
     if (!e) e = mm_map_rows(p.a, p.m, p.k, p.lda, box_a, &map_a);
@@ -716,13 +719,14 @@ cudaError_t go_tc(const SqMatmul& p, int out_type, int split, cudaStream_t st) {
 
 // Which tile and how many parts of k: the least of an estimate, in us, that was
 // fitted to sweeps of 30 shapes from 16 x 512 x 8192 to 256 x 1M x 128 on a B200
-// (the choice is within 10 % of the best of each sweep).  An SM draws what it
-// has in flight per 1.6 us of latency under load, the stages of its resident
-// CTAs, at most 130 bytes a ns; b comes from HBM at 5 TB/s or from L2; a unit's epilogue costs 0.35 us
-// and 1 us per 13000 outputs; a split costs a cluster launch, two cluster barriers and the
-// sums' way through shared memory, and CTAs beyond those that are resident start anew.
-// With few tiles a split is worth much: 64 x 256 x 16384 takes 11.3 us in 8
-// parts, 46 us whole; 256 x 4096 x 4096 14.9 and 17.3 us.
+// (most choices are within a tenth of the best of their sweep).  An SM draws
+// what it has in flight per 1.6 us of latency under load, the stages of its
+// resident CTAs, at most 130 bytes a ns; b comes from HBM at 5 TB/s or from L2;
+// a unit's epilogue costs 0.35 us and 1 us per 13000 outputs; a split costs a
+// cluster launch, two cluster barriers and the sums' way through shared
+// memory, and CTAs beyond those that are resident start anew.  With few tiles a
+// split is worth much: 64 x 256 x 16384 takes 11.3 us in 8 parts, 46 us whole;
+// 256 x 4096 x 4096 14.9 and 17.3 us.
 struct MmPick {
     int nt, split;
     double us;
@@ -772,8 +776,8 @@ bool use_dot(const SqMatmul& p, bool aligned) { return dot_usable(p) && (p.m == 
 // ---- rows that are not 16-byte aligned -------------------------------------
 // The tensor copies need aligned rows; others are copied to scratch whose rows
 // are, 16 bytes a thread.  Putting the rows together inside the product, by
-// warps in the tensor copies' place, took longer (333 x 10007 x 1031: 37 us;
-// 5000^3: 490 us).
+// warps in the tensor copies' place, took longer (333 x 10007 x 1031: 37 us
+// against 26 us; 5000 x 5000 x 5001: 490 us against 177 us).
 int64_t mm_ld(int k) { return (k + 15) / 16 * 16; }
 
 __global__ void __launch_bounds__(256) mm_align_kernel(const int8_t* rows, int64_t n, int k, int64_t ld, int8_t* to,

@@ -254,8 +254,10 @@ cudaError_t sq_read(SqRead p, int type, int bits, cudaStream_t st) {
     return by_type(type, [&](auto t) {
         using T = decltype(t);
         if (bits == 8)
-            return vec ? launch_read<T, 8, kSqVec>(p, st) : words ? launch_shifted<T, 8>(p, st) : launch_read<T, 8, kSqSingle>(p, st);
-        return vec ? launch_read<T, 4, kSqVec>(p, st) : words ? launch_shifted<T, 4>(p, st) : launch_read<T, 4, kSqSingle>(p, st);
+            return vec ? launch_read<T, 8, kSqVec>(p, st)
+                       : words ? launch_shifted<T, 8>(p, st) : launch_read<T, 8, kSqSingle>(p, st);
+        return vec ? launch_read<T, 4, kSqVec>(p, st)
+                   : words ? launch_shifted<T, 4>(p, st) : launch_read<T, 4, kSqSingle>(p, st);
     });
 }
 

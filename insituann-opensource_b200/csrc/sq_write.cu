@@ -143,17 +143,50 @@ __global__ void __launch_bounds__(kSqThreads, CH <= 2 ? 4 : MODE == kSqShifted ?
 }
 
 // Which row stays in a slot that several rows name: claim[slot] = the last of
-// them.  The table needs no contents of its own: the first kernel leaves one
-// row of each named slot there (any of them), the second raises it to the last.
+// them.  The table needs no contents of its own: the first pass leaves one row
+// of each named slot there (any of them), the second raises it to the last.
 // Where no slot is named twice the second finds its own row and writes nothing.
+// Up to kClaimRows rows one cluster runs both passes, with its barrier between
+// them: a launch less (2.3 us of the host; the GPU itself takes 0.8 us longer at
+// 4099 rows, 1.8 us at 10000); more rows need more SMs.
+constexpr uint32_t kClaimRows = 16384;
+constexpr int kClaimCtas = 8, kClaimThreads = 1024;
+
 template <bool RAISE>
-__global__ void sq_claim_kernel(const long long* __restrict__ slots, uint32_t n, uint32_t capacity, int* claim) {
-    for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
-        const uint32_t s = sq_slot(slots, i, capacity);
-        if (s == kNoSlot) continue;
-        if (!RAISE) claim[s] = (int)i;
-        else if (*(volatile int*)(claim + s) < (int)i) atomicMax(claim + s, (int)i);
+__device__ __forceinline__ void sq_claim_pass(const long long* __restrict__ slots, uint32_t n, uint32_t capacity,
+                                              int* claim) {
+    const uint32_t step = gridDim.x * blockDim.x;
+    for (uint32_t i0 = blockIdx.x * blockDim.x + threadIdx.x; i0 < n; i0 += 4 * step) {
+        uint32_t s[4];
+        int c[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[u] = i0 + u * step < n ? sq_slot(slots, i0 + u * step, capacity) : kNoSlot;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (s[u] == kNoSlot) continue;
+            if (!RAISE) claim[s[u]] = (int)(i0 + u * step);
+            else c[u] = *(volatile int*)(claim + s[u]);
+        }
+        if (RAISE) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (s[u] != kNoSlot && c[u] < (int)(i0 + u * step)) atomicMax(claim + s[u], (int)(i0 + u * step));
+        }
     }
+}
+
+template <bool RAISE>
+__global__ void sq_claim_kernel(const long long* slots, uint32_t n, uint32_t capacity, int* claim) {
+    sq_claim_pass<RAISE>(slots, n, capacity, claim);
+}
+
+__global__ void __cluster_dims__(kClaimCtas, 1, 1) __launch_bounds__(kClaimThreads)
+    sq_claim_cluster_kernel(const long long* slots, uint32_t n, uint32_t capacity, int* claim) {
+    sq_claim_pass<false>(slots, n, capacity, claim);
+    __threadfence();
+    __syncthreads();
+    asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+    sq_claim_pass<true>(slots, n, capacity, claim);
 }
 
 int sm_count() {
@@ -220,10 +253,15 @@ cudaError_t sq_write(SqWrite p, int type, int bits, cudaStream_t st) {
     if (!p.group) p.group = p.d;
     p.dedup = !p.slots || p.n == 1 ? kSqAll : p.n <= kSqScanRows ? kSqScan : kSqClaim;
     if (p.dedup == kSqClaim) {
-        const int grid = (int)std::min<int64_t>(((int64_t)p.n + 255) / 256, (int64_t)sm_count() * 16);
-        note_launch(2);
-        sq_claim_kernel<false><<<grid, 256, 0, st>>>(p.slots, p.n, p.capacity, p.claim);
-        sq_claim_kernel<true><<<grid, 256, 0, st>>>(p.slots, p.n, p.capacity, p.claim);
+        if (p.n <= kClaimRows) {
+            note_launch();
+            sq_claim_cluster_kernel<<<kClaimCtas, kClaimThreads, 0, st>>>(p.slots, p.n, p.capacity, p.claim);
+        } else {
+            const int grid = (int)std::min<int64_t>(((int64_t)p.n + 255) / 256, (int64_t)sm_count() * 16);
+            note_launch(2);
+            sq_claim_kernel<false><<<grid, 256, 0, st>>>(p.slots, p.n, p.capacity, p.claim);
+            sq_claim_kernel<true><<<grid, 256, 0, st>>>(p.slots, p.n, p.capacity, p.claim);
+        }
         const cudaError_t e = cudaGetLastError();
         if (e) return e;
     }

@@ -839,6 +839,8 @@ class SQRows:
         self._ldc = codes.stride(0) if n > 1 else max(codes.shape[1], codes.stride(0))
         self._lds = scales.stride(0) if n > 1 else max(scales.shape[1], scales.stride(0))
         self._groups = scales.shape[1]
+        self._claim = None               # scratch of large writes, kept (4 bytes a slot)
+        self._work = {}                  # tokens -> bytes of scratch that scores needs
 
     @property
     def codes(self):
@@ -873,9 +875,13 @@ class SQRows:
         slots = self._slots(slots, n)
         claim = None
         if slots is not None and n > _SQ_SCAN_ROWS:
-            import torch
+            claim = self._claim
+            if claim is None:
+                import torch
 
-            claim = torch.empty(max(self.capacity, 1), dtype=torch.int32, device=self.device)
+                claim = torch.empty(max(self.capacity, 1), dtype=torch.int32, device=self.device)
+                if not torch.cuda.is_current_stream_capturing():     # a graph's memory is the graph's
+                    self._claim = claim
         _sq_call(self.L.ivf_sq_write, self.device, x.data_ptr(), t, n, self.d, ldx,
                  None if slots is None else slots.data_ptr(), self.bits, self.group, self._codes.data_ptr(), self._ldc,
                  self._scales.data_ptr(), self._lds, self.capacity, None if claim is None else claim.data_ptr())
@@ -914,7 +920,11 @@ class SQRows:
         dtype = dtype or (torch.float32 if out is None else out.dtype)
         to = _sq_type(dtype)
         out, ldo = _sq_out(out, m, self.capacity, dtype, self.device)
-        need = self.L.ivf_sq_scores_work(m, self._codes.data_ptr(), self._ldc, self.capacity, self.d)
+        need = self._work.get(m)
+        if need is None:
+            need = self.L.ivf_sq_scores_work(m, self._codes.data_ptr(), self._ldc, self.capacity, self.d)
+            if len(self._work) < 256:
+                self._work[m] = need
         work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         _sq_call(self.L.ivf_sq_scores, self.device, x.data_ptr(), t, ldx, m, self._codes.data_ptr(), self._ldc,
                  self._scales.data_ptr(), self.capacity, self.d, None if bias is None else bias.data_ptr(), out.data_ptr(),
