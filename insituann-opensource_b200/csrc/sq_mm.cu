@@ -274,7 +274,7 @@ struct MmCfg {
     static constexpr int kCols = 2 * NT;                          // tensor-memory columns
     static constexpr int kHalf = NT / (kEpi / 4);                 // columns of an epilogue warp
     static constexpr int kChunk = kHalf < 32 ? kHalf : 32;
-    static constexpr int kStatic = kEpi * kChunk * 4 + 1024;      // static arrays
+    static constexpr int kStatic = kEpi * kHalf * 4 + 1024;       // static arrays
     static constexpr int kFit = (227 * 1024 / kCtas - 1024 - 1024 - kStatic) / kStage;   // 1 KB to align, 1 KB of the system's
     static constexpr int kStages = kFit < kMmMaxStages ? kFit : kMmMaxStages;
     static constexpr size_t kSmem = (size_t)kStage * kStages + 1024;
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
     __shared__ __align__(8) uint64_t bar_ae[2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
-    __shared__ __align__(16) float s_scale[C::kEpi][C::kChunk];
+    __shared__ __align__(16) float s_scale[C::kEpi][C::kHalf];
     const SqMatmul& p = q.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const volatile int* vfail = &s_fail;
@@ -555,9 +555,11 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
         float* sc = s_scale[ew];
         uint32_t n = 0;                                          // tiles done
         bool ok = true;
-        // a tile's place, channel scale and bias are found a tile ahead
+        // a tile's place, scales and bias are found a tile ahead: a load that a
+        // chunk of columns waits for is a good part of its time
+        constexpr int kSa = (C::kHalf + 31) / 32;
         int ct_next = 0, tt_next = 0;
-        float sb_next = 0.f, bias_next = 0.f;
+        float sb_next = 0.f, bias_next = 0.f, sa_next[kSa] = {};
         auto fetch = [&](uint32_t t) {
             mm_place(t, q.tn, q.tm, ct_next, tt_next);
             const int64_t ch = (int64_t)ct_next * kMmM + quarter * 32 + lane;
@@ -565,15 +567,29 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
                 sb_next = p.b_scale[ch];
                 bias_next = p.bias ? p.bias[ch] : 0.f;
             }
+#pragma unroll
+            for (int i = 0; i < kSa; ++i) {
+                const int64_t tok = (int64_t)tt_next * NT + side * C::kHalf + i * 32 + lane;
+                sa_next[i] = tok < p.m ? p.a_scale[tok] : 0.f;
+            }
         };
         if (t0 < tiles) fetch(t0);
         for (uint32_t t = t0; t < tiles; t += gridDim.x, ++n) {
             const int a = (int)(n & 1), tt = tt_next;
             const int64_t ch = (int64_t)ct_next * kMmM + quarter * 32 + lane;
             const float sb = sb_next, bias = bias_next;
+            if (split == 1) {
+#pragma unroll
+                for (int i = 0; i < kSa; ++i)
+                    if (i * 32 + lane < C::kHalf) sc[i * 32 + lane] = sa_next[i];
+            }
             if (t + gridDim.x < tiles) fetch(t + gridDim.x);
             if (ok) ok = __all_sync(0xffffffffu, mm_wait(&bar_af[a], (n / 2) & 1, vfail));
-            if (!ok && lane == 0) s_fail = 1;
+            if (!ok) {
+                if (lane == 0) s_fail = 1;
+                for (int i = lane; i < C::kHalf; i += 32) sc[i] = __int_as_float(0x7fffffff);
+            }
+            __syncwarp();
             tc_fence_after();
             if (split > 1) {
                 // this part's sums to shared memory, [column][channel] (the stages
@@ -604,11 +620,9 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
                 }
                 const int cnt = (int)min((int64_t)C::kChunk, p.m - tok);
                 if (cnt <= 0) continue;
-                if (lane < cnt) sc[lane] = ok ? p.a_scale[tok + lane] : __int_as_float(0x7fffffff);
-                __syncwarp();
-                mm_block(q, tok * p.ldo + ch, v, sc, cnt, sb, bias, (int)min((int64_t)32, p.n - (ch - lane)), lane);
-                __syncwarp();
+                mm_block(q, tok * p.ldo + ch, v, sc + c, cnt, sb, bias, (int)min((int64_t)32, p.n - (ch - lane)), lane);
             }
+            __syncwarp();                                        // sc is read
         }
     }
 
