@@ -492,6 +492,8 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
+    // what was queued before (the kernel that quantised the tokens) is done from here on
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     if (warp == 0) {
         if (lane == 0) {
@@ -721,12 +723,15 @@ cudaError_t go_tc(const SqMatmul& p, int out_type, int split, cudaStream_t st) {
     cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = C::kSmem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)q.split;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    // the kernel may start, and set itself up, while the one before it ends
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     note_launch();
     return cudaLaunchKernelEx(&cfg, mm_tc_kernel<NT>, map_b, map_a, q);
 }
@@ -863,8 +868,15 @@ cudaError_t sq_matmul(SqMatmul p, int out_type, void* work, cudaStream_t st) {
     return e ? e : launch_tc(p, out_type, st);
 }
 
+// Floating tokens: the dot products quantise them themselves, one launch for
+// all.  2 to 4 tokens against much data go to the tensor cores all the same
+// (2 x 911870 x 191: 74 us by dot products, whose warps wait for their loads).
+static bool fused_scores(const SqMatmul& p) {
+    return dot_usable(p) && (p.m == 1 || p.n * p.k <= int64_t(32) << 20 || !rows_aligned(p.b, p.ldb, 16));
+}
+
 size_t sq_scores_work(const SqMatmul& q) {
-    if (q.m == 0 || q.n == 0 || dot_usable(q)) return 0;
+    if (q.m == 0 || q.n == 0 || fused_scores(q)) return 0;
     SqMatmul p = q;
     p.a = nullptr;                                               // the tokens' codes are aligned
     p.lda = mm_ld(p.k);
@@ -873,7 +885,7 @@ size_t sq_scores_work(const SqMatmul& q) {
 
 cudaError_t sq_scores(SqWrite w, int x_type, SqMatmul p, int out_type, void* work, cudaStream_t st) {
     if (p.m == 0 || p.n == 0) return cudaSuccess;
-    if (dot_usable(p)) {
+    if (fused_scores(p)) {
         MmDot q{};
         q.p = p;
         q.x = w.x;

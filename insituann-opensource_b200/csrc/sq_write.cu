@@ -29,6 +29,8 @@ __device__ __forceinline__ bool sq_later(const long long* __restrict__ slots, ui
 template <typename T, int BITS, int MODE, int TEAM, int CH>
 __global__ void __launch_bounds__(kSqThreads, CH > 4 ? 2 : MODE == kSqShifted && CH > 2 ? 3 : 4)
     sq_write_kernel(SqWrite p) {
+    // a product queued behind may set itself up; it waits for this grid's end before it reads
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int E = sq_chunk<T, BITS, MODE>();
     constexpr int TPW = 32 / TEAM;
     const int lane = threadIdx.x & 31, tl = lane % TEAM;
@@ -83,6 +85,7 @@ __global__ void __launch_bounds__(kSqThreads, CH > 4 ? 2 : MODE == kSqShifted &&
 // again, from the caches.
 template <typename T, int BITS, int MODE, int CH>
 __global__ void __launch_bounds__(kSqThreads, CH <= 2 ? 4 : MODE == kSqShifted ? 1 : 3) sq_write_long_kernel(SqWrite p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // as above
     constexpr int E = sq_chunk<T, BITS, MODE>();
     __shared__ uint32_t s_top[kSqThreads / 32];
     const uintptr_t lo = reinterpret_cast<uintptr_t>(p.x), hi = lo + ((uint64_t)(p.n - 1) * p.ldx + p.d) * sizeof(T);

@@ -314,7 +314,8 @@ def test_matmul_output_rows_and_bad_scales(cuda_ok, m):
 
 
 @pytest.mark.parametrize("m,n,d", [(1, 1000, 128), (1, 300, 4096), (2, 77, 96), (4, 129, 1031), (8, 500, 130), (9, 500, 128),
-                                   (33, 1000, 96), (200, 2000, 128), (300, 257, 1000), (3, 40, 20000)])
+                                   (33, 1000, 96), (200, 2000, 128), (300, 257, 1000), (3, 40, 20000),
+                                   (3, 300001, 128)])
 @pytest.mark.parametrize("t", TYPES)
 def test_scores(cuda_ok, m, n, d, t):
     """equal to the product of the rows as write quantises them"""
