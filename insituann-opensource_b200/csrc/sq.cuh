@@ -140,15 +140,39 @@ struct SqBytes {
             }
             const uint4 x = shifted(at);
             uint32_t o[4] = {x.x, x.y, x.z, x.w};
-            if (at + 16 > end) {                                 // clear what follows the row
-                const int left = at < end ? (int)(end - at) : 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int n = left - 4 * i;
-                    o[i] = n >= 4 ? o[i] : n <= 0 ? 0u : o[i] & ((1u << (8 * n)) - 1u);
-                }
-            }
+            if (at + 16 > end) clear(o, at < end ? (int)(end - at) : 0);
             return make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+    // the same for a row with 16 bytes of the array before and behind it, `left` bytes from at to its end (at most
+    // 0: none): no piece leaves the array, and the tests are of 32 bits
+    __device__ __forceinline__ void issue_inner(uintptr_t at, int left) {
+        const uint4* w = reinterpret_cast<const uint4*>(at & ~uintptr_t(15));
+        uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
+        if (left > 0) x = __ldg(w);
+        if (left > 16 - (int)(at & 15)) y = __ldg(w + 1);
+        v[0] = x.x;
+        v[1] = x.y;
+        v[2] = x.z;
+        v[3] = x.w;
+        v[4] = y.x;
+        v[5] = y.y;
+        v[6] = y.z;
+        v[7] = y.w;
+    }
+    __device__ __forceinline__ uint4 take_inner(uintptr_t at, int left) {
+        const uint4 x = shifted(at);
+        if (left >= 16) return x;
+        uint32_t o[4] = {x.x, x.y, x.z, x.w};
+        clear(o, left);
+        return make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    // clears the bytes from `left` on
+    static __device__ __forceinline__ void clear(uint32_t (&o)[4], int left) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = left - 4 * i;
+            o[i] = n >= 4 ? o[i] : n <= 0 ? 0u : o[i] & ((1u << (8 * n)) - 1u);
         }
     }
     // the 16 bytes from at & 15 on: by two words, by one, by bits
@@ -195,12 +219,22 @@ struct SqRaw {
     }
 };
 
+// the bytes of all rows, and whether 16 of them lie before and behind the group at hand
+struct SqSpan {
+    uintptr_t lo, hi;
+    bool inner;
+    template <typename T>
+    __device__ __forceinline__ void at(const T* x, int width) {
+        inner = reinterpret_cast<uintptr_t>(x) - lo >= 16 && hi - reinterpret_cast<uintptr_t>(x + width) >= 16;
+    }
+};
+
 // Values e0 .. e0 + E - 1 of a group of `width` values at x, 0 past its end:
-// issue() starts the loads, take() gives the values.  [lo, hi): all the rows' bytes.
+// issue() starts the loads, take() gives the values.
 template <typename T, int MODE, int E>
 struct SqLoad {
     SqRaw<T, E> r;
-    __device__ __forceinline__ void issue(const T* __restrict__ x, int e0, int width, uintptr_t, uintptr_t) {
+    __device__ __forceinline__ void issue(const T* __restrict__ x, int e0, int width, const SqSpan&) {
 #pragma unroll
         for (int i = 0; i < SqRaw<T, E>::kWords; ++i) r.w[i] = 0;
         if constexpr (MODE == kSqVec) {
@@ -217,17 +251,21 @@ struct SqLoad {
                 }
         }
     }
-    __device__ __forceinline__ SqRaw<T, E> take(const T*, int, int, uintptr_t, uintptr_t) { return r; }
+    __device__ __forceinline__ SqRaw<T, E> take(const T*, int, int, const SqSpan&) { return r; }
 };
 
 template <typename T, int E>
 struct SqLoad<T, kSqShifted, E> {
     SqBytes<false> b;
-    __device__ __forceinline__ void issue(const T* x, int e0, int width, uintptr_t lo, uintptr_t hi) {
-        b.issue(reinterpret_cast<uintptr_t>(x + e0), reinterpret_cast<uintptr_t>(x + width), lo, hi);
+    __device__ __forceinline__ void issue(const T* x, int e0, int width, const SqSpan& s) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(x + e0);
+        if (s.inner) b.issue_inner(at, (width - e0) * (int)sizeof(T));
+        else b.issue(at, reinterpret_cast<uintptr_t>(x + width), s.lo, s.hi);
     }
-    __device__ __forceinline__ SqRaw<T, E> take(const T* x, int e0, int width, uintptr_t lo, uintptr_t hi) {
-        const uint4 v = b.take(reinterpret_cast<uintptr_t>(x + e0), reinterpret_cast<uintptr_t>(x + width), lo, hi);
+    __device__ __forceinline__ SqRaw<T, E> take(const T* x, int e0, int width, const SqSpan& s) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(x + e0);
+        const uint4 v = s.inner ? b.take_inner(at, (width - e0) * (int)sizeof(T))
+                                : b.take(at, reinterpret_cast<uintptr_t>(x + width), s.lo, s.hi);
         SqRaw<T, E> r;
         memcpy(r.w, &v, sizeof(r.w));
         return r;

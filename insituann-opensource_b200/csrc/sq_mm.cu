@@ -60,9 +60,10 @@ __device__ __forceinline__ void dot_quantise(const T* x, int k, uint8_t* codes, 
     constexpr int E = sq_chunk<T, 8, MODE>();
     uint32_t top = 0;
     SqLoad<T, MODE, E> v;
+    const SqSpan span{};                                         // (not used in these modes)
     for (int e0 = threadIdx.x * E; e0 < k; e0 += kDotThreads * E) {
-        v.issue(x, e0, k, 0, 0);
-        v.take(x, e0, k, 0, 0).top(top);
+        v.issue(x, e0, k, span);
+        v.take(x, e0, k, span).top(top);
     }
     top = __reduce_max_sync(0xffffffffu, __float_as_uint(sq_top<T>(top)));
     __syncthreads();
@@ -73,8 +74,8 @@ __device__ __forceinline__ void dot_quantise(const T* x, int k, uint8_t* codes, 
     for (int w = 0; w < kDotThreads / 32; ++w) top = max(top, s_top[w]);
     const SqScale s = sq_scale<8>(__uint_as_float(top));
     for (int e0 = threadIdx.x * E; e0 < k; e0 += kDotThreads * E) {
-        v.issue(x, e0, k, 0, 0);
-        sq_store<T, 8, MODE, E>(codes, e0, k, v.take(x, e0, k, 0, 0), s);
+        v.issue(x, e0, k, span);
+        sq_store<T, 8, MODE, E>(codes, e0, k, v.take(x, e0, k, span), s);
     }
     if (threadIdx.x == 0) *scale = s.scale;
 }

@@ -35,7 +35,9 @@ __global__ void __launch_bounds__(kSqThreads, CH > 4 ? 2 : MODE == kSqShifted &&
     constexpr int TPW = 32 / TEAM;
     const int lane = threadIdx.x & 31, tl = lane % TEAM;
     const uint32_t tmask = (TEAM == 32 ? 0xffffffffu : (1u << (TEAM & 31)) - 1u) << (lane / TEAM * TEAM);
-    const uintptr_t lo = reinterpret_cast<uintptr_t>(p.x), hi = lo + ((uint64_t)(p.n - 1) * p.ldx + p.d) * sizeof(T);
+    SqSpan span;
+    span.lo = reinterpret_cast<uintptr_t>(p.x);
+    span.hi = span.lo + ((uint64_t)(p.n - 1) * p.ldx + p.d) * sizeof(T);
     const uint64_t items = (uint64_t)p.n * (uint32_t)p.groups;
     const uint64_t warp0 = (uint64_t)blockIdx.x * (kSqThreads / 32) + (threadIdx.x >> 5);
     for (uint64_t base = warp0 * TPW; base < items; base += (uint64_t)gridDim.x * (kSqThreads / 32 * TPW)) {
@@ -47,9 +49,10 @@ __global__ void __launch_bounds__(kSqThreads, CH > 4 ? 2 : MODE == kSqShifted &&
         const int e_lo = g * p.group;
         const int width = live ? min(p.group, p.d - e_lo) : 0;
         const T* xr = static_cast<const T*>(p.x) + (uint64_t)row * p.ldx + e_lo;
+        span.at(xr, width);
         SqLoad<T, MODE, E> in[CH];
 #pragma unroll
-        for (int c = 0; c < CH; ++c) in[c].issue(xr, (tl + c * TEAM) * E, width, lo, hi);
+        for (int c = 0; c < CH; ++c) in[c].issue(xr, (tl + c * TEAM) * E, width, span);
         uint32_t slot = live ? sq_slot(p.slots, row, p.capacity) : kNoSlot;
         if (p.dedup == kSqClaim) {
             if (slot != kNoSlot && (uint32_t)p.claim[slot] != row) slot = kNoSlot;
@@ -62,7 +65,7 @@ __global__ void __launch_bounds__(kSqThreads, CH > 4 ? 2 : MODE == kSqShifted &&
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             if (MODE == kSqShifted && c * TEAM * E >= width) break;
-            v[c] = in[c].take(xr, (tl + c * TEAM) * E, width, lo, hi);
+            v[c] = in[c].take(xr, (tl + c * TEAM) * E, width, span);
             v[c].top(top);
         }
         top = __float_as_uint(sq_top<T>(top));
@@ -84,11 +87,13 @@ __global__ void __launch_bounds__(kSqThreads, CH > 4 ? 2 : MODE == kSqShifted &&
 // keeps its first CH chunks; what a group has beyond kSqThreads * CH is read
 // again, from the caches.
 template <typename T, int BITS, int MODE, int CH>
-__global__ void __launch_bounds__(kSqThreads, CH <= 2 ? 4 : MODE == kSqShifted ? 1 : 3) sq_write_long_kernel(SqWrite p) {
+__global__ void __launch_bounds__(kSqThreads, CH <= 2 ? 4 : MODE == kSqShifted ? CH <= 4 ? 2 : 1 : 3) sq_write_long_kernel(SqWrite p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // as above
     constexpr int E = sq_chunk<T, BITS, MODE>();
     __shared__ uint32_t s_top[kSqThreads / 32];
-    const uintptr_t lo = reinterpret_cast<uintptr_t>(p.x), hi = lo + ((uint64_t)(p.n - 1) * p.ldx + p.d) * sizeof(T);
+    SqSpan span;
+    span.lo = reinterpret_cast<uintptr_t>(p.x);
+    span.hi = span.lo + ((uint64_t)(p.n - 1) * p.ldx + p.d) * sizeof(T);
     const uint64_t items = (uint64_t)p.n * (uint32_t)p.groups;
     for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
         uint32_t row = 0;
@@ -97,10 +102,11 @@ __global__ void __launch_bounds__(kSqThreads, CH <= 2 ? 4 : MODE == kSqShifted ?
         const int e_lo = g * p.group;
         const int width = min(p.group, p.d - e_lo);
         const T* xr = static_cast<const T*>(p.x) + (uint64_t)row * p.ldx + e_lo;
+        span.at(xr, width);
         SqLoad<T, MODE, E> in[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c)
-            if (MODE == kSqVec || c * kSqThreads * E < width) in[c].issue(xr, ((int)threadIdx.x + c * kSqThreads) * E, width, lo, hi);
+            if (MODE == kSqVec || c * kSqThreads * E < width) in[c].issue(xr, ((int)threadIdx.x + c * kSqThreads) * E, width, span);
         uint32_t slot = sq_slot(p.slots, row, p.capacity);
         bool later = false;
         if (p.dedup == kSqClaim) {
@@ -113,13 +119,13 @@ __global__ void __launch_bounds__(kSqThreads, CH <= 2 ? 4 : MODE == kSqShifted ?
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             if (MODE != kSqVec && c * kSqThreads * E >= width) break;
-            v[c] = in[c].take(xr, ((int)threadIdx.x + c * kSqThreads) * E, width, lo, hi);
+            v[c] = in[c].take(xr, ((int)threadIdx.x + c * kSqThreads) * E, width, span);
             v[c].top(top);
         }
         for (int e0 = ((int)threadIdx.x + CH * kSqThreads) * E; e0 < width; e0 += kSqThreads * E) {
             SqLoad<T, MODE, E> more;
-            more.issue(xr, e0, width, lo, hi);
-            more.take(xr, e0, width, lo, hi).top(top);
+            more.issue(xr, e0, width, span);
+            more.take(xr, e0, width, span).top(top);
         }
         top = __reduce_max_sync(0xffffffffu, __float_as_uint(sq_top<T>(top)));
         if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
@@ -138,8 +144,8 @@ __global__ void __launch_bounds__(kSqThreads, CH <= 2 ? 4 : MODE == kSqShifted ?
         }
         for (int e0 = ((int)threadIdx.x + CH * kSqThreads) * E; e0 < width; e0 += kSqThreads * E) {
             SqLoad<T, MODE, E> more;
-            more.issue(xr, e0, width, lo, hi);
-            sq_store<T, BITS, MODE, E>(cr, e0, width, more.take(xr, e0, width, lo, hi), s);
+            more.issue(xr, e0, width, span);
+            sq_store<T, BITS, MODE, E>(cr, e0, width, more.take(xr, e0, width, span), s);
         }
         if (threadIdx.x == 0) p.scales[(uint64_t)slot * p.lds + g] = s.scale;
     }
@@ -242,6 +248,8 @@ cudaError_t launch_write(const SqWrite& p, cudaStream_t st) {
     const int grid = (int)std::min<int64_t>((int64_t)p.n * p.groups, (int64_t)sm_count() * 8);
     note_launch();
     if (chunks <= 2 * kSqThreads) sq_write_long_kernel<T, BITS, MODE, 2><<<grid, kSqThreads, 0, st>>>(p);
+    else if (MODE == kSqShifted && chunks <= 4 * kSqThreads)
+        sq_write_long_kernel<T, BITS, MODE, MODE == kSqShifted ? 4 : 8><<<grid, kSqThreads, 0, st>>>(p);
     else sq_write_long_kernel<T, BITS, MODE, 8><<<grid, kSqThreads, 0, st>>>(p);
     return cudaGetLastError();
 }
