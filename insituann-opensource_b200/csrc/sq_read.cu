@@ -205,6 +205,7 @@ cudaError_t launch_read(const SqRead& p, cudaStream_t st) {
         if (chunks > 16 && chunks <= 24) return go_read<T, BITS, MODE, 8, 3, 2>(p, st);
         if (chunks > 24 && chunks <= 32) return go_read<T, BITS, MODE, 8, 4, 2>(p, st);
         if (chunks > 4 && chunks <= 16) return go_read<T, BITS, MODE, 4, 4, 2>(p, st);
+        if (chunks > 32 && chunks <= 64) return go_read<T, BITS, MODE, 16, 4, 1>(p, st);
     } else {
         // neighbouring lanes store neighbouring values
         if (chunks > 4 && chunks <= 8) return go_read<T, BITS, MODE, 8, 1, 4>(p, st);
@@ -231,8 +232,8 @@ cudaError_t launch_shifted(const SqRead& p, cudaStream_t st) {
     if (chunks <= 4) return go_shifted<T, BITS, 4, 1, 4>(p, st);
     if (chunks <= 8) return go_shifted<T, BITS, 4, 2, 2>(p, st);
     if (chunks <= 16) return go_shifted<T, BITS, 8, 2, 2>(p, st);
-    if (chunks <= 32) return go_shifted<T, BITS, 16, 2, 2>(p, st);
-    return go_shifted<T, BITS, 32, 4, 1>(p, st);
+    if (chunks <= 64) return go_shifted<T, BITS, 16, 2, 2>(p, st);
+    return go_shifted<T, BITS, 32, 2, 2>(p, st);
 }
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }

@@ -20,6 +20,7 @@ constexpr int kSqThreads = 256;
 __device__ __forceinline__ bool sq_later(const long long* __restrict__ slots, uint32_t n, uint32_t row, uint32_t slot,
                                          int lane, int team) {
     bool later = false;
+#pragma unroll 4
     for (uint32_t j = row + 1 + lane; j < n; j += team) later |= slots[j] == (long long)slot;
     return later;
 }
