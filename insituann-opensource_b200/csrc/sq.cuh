@@ -219,6 +219,14 @@ struct SqRaw {
     }
 };
 
+// 16 bytes at the ends of the array, out of line: the first and the last row
+// take this way only, and a small call's time is reading its instructions
+static __device__ __noinline__ uint4 sq_end_bytes(uintptr_t at, uintptr_t end, uintptr_t lo, uintptr_t hi) {
+    SqBytes<false> b;
+    b.issue(at, end, lo, hi);
+    return b.take(at, end, lo, hi);
+}
+
 // the bytes of all rows, and whether 16 of them lie before and behind the group at hand
 struct SqSpan {
     uintptr_t lo, hi;
@@ -259,13 +267,12 @@ struct SqLoad<T, kSqShifted, E> {
     SqBytes<false> b;
     __device__ __forceinline__ void issue(const T* x, int e0, int width, const SqSpan& s) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(x + e0);
-        if (s.inner) b.issue_inner(at, (width - e0) * (int)sizeof(T));
-        else b.issue(at, reinterpret_cast<uintptr_t>(x + width), s.lo, s.hi);
+        b.issue_inner(at, s.inner ? (width - e0) * (int)sizeof(T) : 0);
     }
     __device__ __forceinline__ SqRaw<T, E> take(const T* x, int e0, int width, const SqSpan& s) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(x + e0);
-        const uint4 v = s.inner ? b.take_inner(at, (width - e0) * (int)sizeof(T))
-                                : b.take(at, reinterpret_cast<uintptr_t>(x + width), s.lo, s.hi);
+        uint4 v = b.take_inner(at, (width - e0) * (int)sizeof(T));
+        if (!s.inner && e0 < width) v = sq_end_bytes(at, reinterpret_cast<uintptr_t>(x + width), s.lo, s.hi);
         SqRaw<T, E> r;
         memcpy(r.w, &v, sizeof(r.w));
         return r;

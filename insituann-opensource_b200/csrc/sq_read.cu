@@ -81,6 +81,13 @@ __global__ void __launch_bounds__(kSqThreads) sq_read_kernel(SqRead p) {
     }
 }
 
+// the last word of a store's last row, of which `n` bytes are there
+__device__ __noinline__ uint32_t sq_last_word(const uint8_t* at, int n) {
+    uint32_t w = 0;
+    for (int k = 0; k < n && k < 4; ++k) w |= (uint32_t)at[k] << (8 * k);
+    return w;
+}
+
 // The same for output rows that are not aligned (an odd d, a slice): chunks are
 // 16 aligned bytes of output, so a row's first and last chunk may be a part (stored value by
 // value) and a chunk's codes start anywhere, at a nibble too: they are shifted
@@ -129,8 +136,7 @@ __global__ void __launch_bounds__(kSqThreads) sq_read_shifted_kernel(SqRead p) {
                             // the store may end inside its last row's last word
                             if (b + 4 <= bytes || slot[r] + 1 < p.capacity)
                                 w[r][c][i] = *reinterpret_cast<const uint32_t*>(codes[r] + b);
-                            else
-                                for (int k = 0; b + k < bytes; ++k) w[r][c][i] |= (uint32_t)codes[r][b + k] << (8 * k);
+                            else w[r][c][i] = sq_last_word(codes[r] + b, bytes - b);
                         }
                     }
                     s0[r][c] = s1[r][c] = 0.f;
@@ -233,7 +239,8 @@ cudaError_t launch_shifted(const SqRead& p, cudaStream_t st) {
     if (chunks <= 8) return go_shifted<T, BITS, 4, 2, 2>(p, st);
     if (chunks <= 16) return go_shifted<T, BITS, 8, 2, 2>(p, st);
     if (chunks <= 64) return go_shifted<T, BITS, 16, 2, 2>(p, st);
-    return go_shifted<T, BITS, 32, 2, 2>(p, st);
+    if (chunks <= 128) return go_shifted<T, BITS, 32, 2, 2>(p, st);
+    return go_shifted<T, BITS, 32, 4, 1>(p, st);
 }
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
