@@ -839,7 +839,8 @@ class SQRows:
         self._ldc = codes.stride(0) if n > 1 else max(codes.shape[1], codes.stride(0))
         self._lds = scales.stride(0) if n > 1 else max(scales.shape[1], scales.stride(0))
         self._groups = scales.shape[1]
-        self._claim = None               # scratch of large writes, kept (4 bytes a slot)
+        self._claim = None               # scratch of large writes, kept (4 bytes a slot), and the stream it is of
+        self._claim_stream = None
         self._work = {}                  # tokens -> bytes of scratch that scores needs
 
     @property
@@ -875,13 +876,19 @@ class SQRows:
         slots = self._slots(slots, n)
         claim = None
         if slots is not None and n > _SQ_SCAN_ROWS:
-            claim = self._claim
-            if claim is None:
-                import torch
+            import torch
 
+            # a captured write takes scratch of its own: the graph may run beside others, and outlive the store
+            capturing = torch.cuda.is_current_stream_capturing()
+            claim = None if capturing else self._claim
+            if claim is None:
                 claim = torch.empty(max(self.capacity, 1), dtype=torch.int32, device=self.device)
-                if not torch.cuda.is_current_stream_capturing():     # a graph's memory is the graph's
+                if not capturing:
                     self._claim = claim
+                    self._claim_stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+            elif torch._C._cuda_getCurrentRawStream(self.device.index) != self._claim_stream:
+                # the store may be dropped while this write runs: its scratch is not handed out before it ends
+                claim.record_stream(torch.cuda.current_stream(self.device))
         _sq_call(self.L.ivf_sq_write, self.device, x.data_ptr(), t, n, self.d, ldx,
                  None if slots is None else slots.data_ptr(), self.bits, self.group, self._codes.data_ptr(), self._ldc,
                  self._scales.data_ptr(), self._lds, self.capacity, None if claim is None else claim.data_ptr())

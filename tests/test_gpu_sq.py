@@ -411,6 +411,54 @@ def test_graph_and_streams(cuda_ok):
     assert not torch.equal(y2, warm[0])
 
 
+def test_write_scratch_outlives_the_store(cuda_ok):
+    """a large write on another stream than the first one's, the store dropped while it waits: its scratch is
+    not handed out to others before it has run"""
+    n, cap = 2000, 1 << 20
+    gen = torch.Generator().manual_seed(5)
+    x = torch.randn(n, 32, generator=gen).cuda()
+    slots = torch.randint(0, cap, (n,), generator=gen).cuda()
+    codes = torch.zeros(cap, 32, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(cap, 1, device="cuda")
+    rows = ib.SQRows.from_arrays(codes, scales, 32)
+    rows.write(x, slots)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        rows.write(x, slots)
+    del rows
+    others = [torch.full((cap,), -7, dtype=torch.int32, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    for o in others:
+        assert bool((o == -7).all())
+
+
+def test_captured_write_outlives_the_store(cuda_ok):
+    """a graph of a large write, replayed after its store is gone: the scratch is the graph's own"""
+    n, cap = 2000, 1 << 20
+    gen = torch.Generator().manual_seed(6)
+    x = torch.randn(n, 32, generator=gen).cuda()
+    slots = torch.randint(0, cap, (n,), generator=gen).cuda()
+    codes = torch.zeros(cap, 32, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(cap, 1, device="cuda")
+    rows = ib.SQRows.from_arrays(codes, scales, 32)
+    rows.write(x, slots)
+    want = codes.clone(), scales.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rows.write(x, slots)
+    del rows
+    codes.zero_()
+    scales.zero_()
+    others = [torch.full((cap,), -7, dtype=torch.int32, device="cuda") for _ in range(4)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(codes, want[0]) and torch.equal(scales, want[1])
+    for o in others:
+        assert bool((o == -7).all())
+
+
 def test_binding_refusals(cuda_ok):
     store = ib.SQRows(10, 32)
     x = torch.randn(4, 32, device="cuda")
