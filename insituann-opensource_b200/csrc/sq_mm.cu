@@ -797,41 +797,69 @@ bool use_dot(const SqMatmul& p, bool aligned) { return dot_usable(p) && (p.m == 
 // The tensor copies need aligned rows; others are copied to scratch whose rows
 // are, 16 bytes a thread.  Putting the rows together inside the product, by
 // warps in the tensor copies' place, took longer (333 x 10007 x 1031: 37 us
-// against 26 us; 5000 x 5000 x 5001: 490 us against 177 us).
-int64_t mm_ld(int k) { return (k + 15) / 16 * 16; }
+// against 17 us; 5000 x 5000 x 5001: 490 us against 127 us).
+// Scratch rows are whole 32-byte sectors (333 x 10007 x 1031: 10 us for the product, 13 us with rows of 1040
+// bytes) but for short ones, to which that would add a fourth and more.
+int64_t mm_ld(int k) { return k <= 64 ? (k + 15) / 16 * 16 : (k + 31) / 32 * 32; }
 
-__global__ void __launch_bounds__(256) mm_align_kernel(const int8_t* rows, int64_t n, int k, int64_t ld, int8_t* to,
-                                                       int64_t ldt) {
-    const uintptr_t lo = reinterpret_cast<uintptr_t>(rows), hi = lo + (n - 1) * ld + k;
-    const int chunks = (int)(ldt / 16);
-    const uint64_t items = (uint64_t)n * chunks, step = (uint64_t)gridDim.x * 256 * 4;
-    for (uint64_t i0 = (uint64_t)blockIdx.x * 256 * 4 + threadIdx.x; i0 < items; i0 += step) {
-        SqBytes<false> raw[4];
-        uintptr_t at[4], end[4];
-        int8_t* out[4];
+// Both operands in one launch (blockIdx.y).  A block takes `rows_at_once` rows, about
+// 4 chunks a thread: rows are found by one multiplication, from the
+// block's first (a division and 64-bit products per chunk took 10.6 us for the
+// 10340 rows of 1031 bytes of the first product above).
+struct MmAlign {
+    const int8_t* rows[2];
+    int64_t n[2], ld[2];
+    int8_t* to[2];
+    int k, chunks;              // 16-byte pieces of a row in scratch
+    uint32_t inverse;           // ceil(2^32 / chunks): exact quotients of numbers below 2^19
+    int rows_at_once;
+};
+constexpr int kAlignChunks = 4 * 256;
+
+__global__ void __launch_bounds__(256) mm_align_kernel(const __grid_constant__ MmAlign p) {
+    // the product may set itself up meanwhile; it waits for this grid's end before it reads
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int y = blockIdx.y;
+    const int64_t n = p.n[y], ld = p.ld[y], last = (n - 1) * ld;
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p.rows[y]);
+    for (int64_t row0 = (int64_t)blockIdx.x * p.rows_at_once; row0 < n; row0 += (int64_t)gridDim.x * p.rows_at_once) {
+        const int64_t first = row0 * ld;
+        const int items = (int)min((int64_t)p.rows_at_once, n - row0) * p.chunks;
+        uint4* const out = reinterpret_cast<uint4*>(p.to[y]) + row0 * p.chunks;
+        for (int t0 = threadIdx.x; t0 < items; t0 += kAlignChunks) {
+            SqBytes<false> raw[4];
+            uintptr_t at[4];
+            int left[4];
+            bool inner[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            uint32_t row = 0;
-            int c = 0;
-            const bool in = i0 + u * 256 < items;
-            sq_split(in ? i0 + u * 256 : 0, chunks, row, c);
-            const uintptr_t first = lo + (int64_t)row * ld;
-            at[u] = first + 16 * c;
-            end[u] = in ? first + k : 0;
-            out[u] = in ? to + (int64_t)row * ldt + 16 * c : nullptr;
-            raw[u].issue(at[u], end[u], lo, hi);
+            for (int u = 0; u < 4; ++u) {
+                const int t = t0 + u * 256;
+                const uint32_t r = p.chunks == 1 ? t : __umulhi((uint32_t)t, p.inverse);
+                const int c = t - (int)r * p.chunks;
+                const int64_t before = first + (int64_t)r * (uint32_t)ld;
+                at[u] = lo + before + 16 * c;
+                left[u] = t < items ? p.k - 16 * c : 0;          // not above 0: a piece behind the row's end
+                inner[u] = before >= 16 && last - before >= 16;  // so many bytes lie before and behind the row
+                raw[u].issue_inner(at[u], inner[u] ? left[u] : 0);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (t0 + u * 256 >= items) continue;
+                uint4 v = raw[u].take_inner(at[u], left[u]);
+                if (!inner[u] && left[u] > 0) v = sq_end_bytes(at[u], at[u] + left[u], lo, lo + last + p.k);
+                out[t0 + u * 256] = v;
+            }
         }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (out[u]) *reinterpret_cast<uint4*>(out[u]) = raw[u].take(at[u], end[u], lo, hi);
     }
 }
 
-cudaError_t launch_align(const int8_t* rows, int64_t n, int k, int64_t ld, int8_t* to, cudaStream_t st) {
-    const int64_t items = n * (mm_ld(k) / 16), per = 256 * 4;
+cudaError_t launch_align(MmAlign& p, cudaStream_t st) {
+    p.chunks = (int)(mm_ld(p.k) / 16);
+    p.inverse = p.chunks == 1 ? 0 : (uint32_t)(((uint64_t(1) << 32) + p.chunks - 1) / p.chunks);
+    p.rows_at_once = std::max(1, kAlignChunks / p.chunks);
+    const int64_t blocks = (std::max(p.n[0], p.n[1]) + p.rows_at_once - 1) / p.rows_at_once;
     note_launch();
-    mm_align_kernel<<<(int)std::min<int64_t>((items + per - 1) / per, (int64_t)sm_count() * 16), 256, 0, st>>>(
-        rows, n, k, ld, to, mm_ld(k));
+    mm_align_kernel<<<dim3((unsigned)std::min<int64_t>(blocks, (int64_t)sm_count() * 16), p.n[1] ? 2 : 1), 256, 0, st>>>(p);
     return cudaGetLastError();
 }
 
@@ -853,19 +881,23 @@ cudaError_t sq_matmul(SqMatmul p, int out_type, void* work, cudaStream_t st) {
         q.out_type = out_type;
         return launch_dot(q, st);
     }
+    if (al_a && al_b) return launch_tc(p, out_type, st);
+    MmAlign q{};
+    q.k = p.k;
     int8_t* to = static_cast<int8_t*>(work);
-    cudaError_t e = cudaSuccess;
-    if (!al_b) {
-        e = launch_align(p.b, p.n, p.k, p.ldb, to, st);
-        p.b = to;
-        p.ldb = mm_ld(p.k);
-        to += p.n * p.ldb;
-    }
-    if (!e && !al_a) {
-        e = launch_align(p.a, p.m, p.k, p.lda, to, st);
-        p.a = to;
-        p.lda = mm_ld(p.k);
-    }
+    int i = 0;
+    auto copied = [&](const int8_t*& rows, int64_t n, int64_t& ld) {
+        q.rows[i] = rows;
+        q.n[i] = n;
+        q.ld[i] = ld;
+        q.to[i++] = to;
+        rows = to;
+        ld = mm_ld(p.k);
+        to += n * ld;
+    };
+    if (!al_b) copied(p.b, p.n, p.ldb);
+    if (!al_a) copied(p.a, p.m, p.lda);
+    const cudaError_t e = launch_align(q, st);
     return e ? e : launch_tc(p, out_type, st);
 }
 
