@@ -336,7 +336,7 @@ __device__ __forceinline__ void sq_codes(const SqRaw<T, E>& x, const SqScale& s,
         const float v = x.get(0);
         const float t = __fmaf_rn(v, s.inv, kMagic);
         k[0] = __float_as_uint(t);
-        far = fabsf(__fmaf_rn(kMagic - t, s.scale, v));
+        far = fmaxf(far, fabsf(__fmaf_rn(kMagic - t, s.scale, v)));
     } else {
         const float2 inv = make_float2(s.inv, s.inv), sc = make_float2(-s.scale, -s.scale);
 #pragma unroll
