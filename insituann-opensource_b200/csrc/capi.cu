@@ -1450,7 +1450,7 @@ void sq_check_store(const void* codes, long long ldc, const float* scales, long 
     need(group == 0 || (group > 0 && group % 16 == 0), "group must be 0 or a multiple of 16");
     need(capacity >= 0 && capacity < 2147483647ll, "need 0 <= capacity < 2^31 - 1");
     need(ldc >= (d * (long long)bits + 7) / 8 && ldc < (1ll << 32), "ldc is below a row's bytes (or above 2^32)");
-    need(lds >= (group ? (d + group - 1) / group : 1) && lds < (1ll << 32),
+    need(lds >= (group ? ((long long)d + group - 1) / group : 1) && lds < (1ll << 32),
             "lds is below a row's number of scales (or above 2^32)");
     need(capacity == 0 || (codes && scales), "null pointer");
     need(reinterpret_cast<uintptr_t>(scales) % 4 == 0, "scales must be 4-byte aligned");
