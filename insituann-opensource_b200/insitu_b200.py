@@ -820,7 +820,7 @@ class SQRows:
 
         _sq_need(bits in (8, 4), "bits must be 8 or 4")
         _sq_need(1 <= d <= 1 << 20, "need 1 <= d <= 2^20")
-        _sq_need(group >= 0 and group % 16 == 0, "group must be 0 or a multiple of 16")
+        _sq_need(0 <= group < 1 << 31 and group % 16 == 0, "group must be 0 or a multiple of 16 below 2^31")
         _sq_need(codes.dim() == 2 and scales.dim() == 2 and codes.shape[0] == scales.shape[0],
                  "codes and scales must be 2-D with a row per slot")
         _sq_need(codes.is_cuda and scales.device == codes.device, "codes and scales must be on one CUDA device")

@@ -33,3 +33,13 @@ def test_rows_have_room_for_their_scales(call, group, d):
     rows = dict(d=d, ldx=d) if call is write else dict(d=d, ldo=d)
     for lds, rc in ((least, OK), (least + 5, OK), (least - 1, EINVAL), (0, EINVAL), (-1, EINVAL)):
         assert call(group=group, lds=lds, ldc=d, **rows) == rc, lds
+
+
+@pytest.mark.parametrize("group", [1 << 31, (1 << 32) + 16, 1 << 40])
+def test_binding_refuses_groups_that_no_int_holds(group):
+    """(ctypes would pass their last 32 bits on: a group of 16, with more scales than the store has room for)"""
+    import torch
+
+    rows = ib.SQRows.__new__(ib.SQRows)
+    with pytest.raises(ValueError, match="group"):
+        rows._adopt(torch.zeros(4, 32, dtype=torch.int8), torch.zeros(4, 8)[:, :1], 20, 8, group)
