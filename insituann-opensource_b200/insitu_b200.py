@@ -728,6 +728,16 @@ def _sq_out(out, n, d, dtype, device):
     return out, (ld if n > 1 and ld > 0 else max(d, 1))
 
 
+def _sq_capturing(device):
+    """whether torch's current stream of that device, the one that _sq_call uses, is being captured"""
+    import torch
+
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return torch.cuda.is_current_stream_capturing()
+    return torch.cuda.is_current_stream_capturing()
+
+
 def _sq_call(fn, device, *args):
     """fn(*args, stream) with the tensors' device current, on torch's current stream of that device"""
     import torch
@@ -879,7 +889,7 @@ class SQRows:
             import torch
 
             # a captured write takes scratch of its own: the graph may run beside others, and outlive the store
-            capturing = torch.cuda.is_current_stream_capturing()
+            capturing = _sq_capturing(self.device)
             claim = None if capturing else self._claim
             if claim is None:
                 claim = torch.empty(max(self.capacity, 1), dtype=torch.int32, device=self.device)
