@@ -23,8 +23,8 @@
  *     read with ivf_last_error().
  * No function aborts, exits or resets the device.
  *
- * Environment (read on every call; every choice gives the same results bit
- * for bit):
+ * Environment (read on every call; every choice, but for a short
+ * INSITU_SQ_WAIT_NS, gives the same results bit for bit):
  *   INSITU_SCRATCH_MB   per-batch scratch budget in MB (default: an eighth
  *                       of the device's memory, 1 to 24 GB); larger batches
  *                       run in query sub-batches inside one call
@@ -41,6 +41,10 @@
  *                       own tiles after each list's main rows; unset:
  *                       "direct" up to 100 delta rows per list on average,
  *                       else "mix"
+ *   INSITU_SQ_WAIT_NS   the limit of a wait inside an 8-bit product, in ns (at
+ *                       most, and unset, 2 s): after it the product gives
+ *                       up, and ivf_sq_status reports it (0: without
+ *                       waiting, to try out how a program takes the error)
  *
  * Citations are paths inside the reference project
  * (mindtravel/InSituANN-OpenSource).
@@ -337,7 +341,8 @@ int ivf_pq_encode(const void* d_x, int x_is_u8, long long n, int d, const int* d
  * Arrays of floating values are aligned to their type, d_slots to 8 bytes;
  * 16-byte aligned rows are fastest.  An output must not overlap an input.  Two calls that write one
  * store (or use one d_claim or d_work) must be ordered.  Failures are
- * reported through ivf_global_last_error().
+ * reported through ivf_global_last_error(); one that shows on the device only, a wait
+ * inside a product that gave up after 2 s, is reported by ivf_sq_status().
  * ====================================================================== */
 /* types of floating rows */
 #define IVF_SQ_F32 0
@@ -392,6 +397,13 @@ int ivf_sq_scores(const void* d_x, int x_type, long long ldx, long long m, const
                   long long ldo, void* d_work, size_t work_bytes, void* stream);
 /* bytes of d_work that ivf_sq_scores needs for this store (0 for sizes that it refuses) */
 size_t ivf_sq_scores_work(long long m, const int8_t* d_codes, long long ldc, long long n, int d);
+/*
+ * Waits for the work queued on `stream` and returns IVF_ECUDA when a product
+ * (ivf_sq_matmul, ivf_sq_scores) that has run on the current device, on any
+ * stream, gave up a wait on the device since the last such report: its outputs
+ * are not valid.  Not for a stream that is being captured.
+ */
+int ivf_sq_status(void* stream);
 
 /* ======================================================================
  * Update overlay (new: runner-internal in the reference,

@@ -1604,6 +1604,18 @@ size_t ivf_sq_scores_work(long long m, const int8_t* d_codes, long long ldc, lon
     return sq_scores_work(p);
 }
 
+int ivf_sq_status(void* stream) {
+    return guarded(nullptr, [&] {
+        const auto st = static_cast<cudaStream_t>(stream);
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        ck(cudaStreamIsCapturing(st, &capture), "stream");
+        need(capture == cudaStreamCaptureStatusNone, "the stream is being captured");
+        bool gave_up = false;
+        ck(sq_status(&gave_up, st), "sq_status");
+        if (gave_up) fail(IVF_ECUDA, "a bounded device wait of an 8-bit product gave up: its outputs are not valid");
+    });
+}
+
 int ivf_set_shard(void* idx_ctx, int nlist_global, const int* local_to_global, const long long* key_offsets) {
     IndexCtx* x = nullptr;
     try {

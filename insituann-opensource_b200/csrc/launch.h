@@ -269,6 +269,8 @@ struct SqMatmul {
 };
 // work: sq_matmul_work(p) bytes, 16-byte aligned (for rows that are not)
 size_t sq_matmul_work(const SqMatmul& p);
+// waits for st; whether a product on the current device gave up a wait since the last report
+cudaError_t sq_status(bool* gave_up, cudaStream_t st);
 cudaError_t sq_matmul(SqMatmul p, int out_type, void* work, cudaStream_t st);
 // the product of the floating rows of w (x_type; only x, n, ldx, d are given),
 // quantised one scale a row; p without its tokens but for m

@@ -5,6 +5,7 @@
 // rounded once more, to its type.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <type_traits>
 
 #include "launch.h"
@@ -261,8 +262,9 @@ cudaError_t launch_dot(MmDot q, cudaStream_t st) {
 // The parts of a split tile are the CTAs of one cluster: each leaves its sums in
 // its shared memory and adds up, over the cluster, the columns that fall to
 // it (whole numbers: the order does not matter).
-// Every wait on a barrier in memory is bounded; after one that gives up the CTA's
-// remaining outputs are NaN.
+// Every wait on a barrier in memory is bounded; a CTA in which one gives up raises
+// g_mm_gave_up (its outputs are not valid then: what it still stores is NaN
+// mostly), lets its copies and MMAs in flight end, and returns.
 constexpr int kMmM = 128, kMmK = 128;
 constexpr int kMmMaxStages = 12;
 
@@ -291,10 +293,20 @@ __device__ __forceinline__ void mm_place(uint32_t t, uint32_t tn, uint32_t tm, i
     tt = (int)(8 * band + r - (uint32_t)ct * w);
 }
 
-// wait on an mbarrier phase, suspended, bounded by kTCWaitNs of wall time; false where it gave up
-__device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, const volatile int* fail) {
-    if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
-    return mbar_wait_timed(bar, parity, fail);
+// set by a product with a wait that gave up, read and cleared by sq_status
+__device__ int g_mm_gave_up;
+
+// Wait on an mbarrier phase, suspended, bounded by `limit` ns of wall time; false
+// where it gave up, early once *fail is set (fail may be null).  A limit of 0 polls only.
+__device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, const volatile int* fail, uint32_t limit) {
+    if (mbar_try_wait_sleep(bar, parity, min(limit, 20000u))) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (;;) {
+        if (fail && *fail) return false;
+        const bool over = globaltimer_ns() - t0 >= limit;
+        if (mbar_try_wait_sleep(bar, parity, over ? 0u : 20000u)) return true;
+        if (over) return false;
+    }
 }
 
 // The copying and the MMA thread run once per 128 bytes of k, some 500 clocks of
@@ -310,12 +322,12 @@ struct MmRing {
     }
 };
 
-// waits until every phase of a ring's stages that was begun is over
+// waits, for kTCWaitNs each, until every phase of a ring's stages that was begun is over
 __device__ __forceinline__ void mm_drain(uint64_t* bars, MmRing r, uint32_t stages) {
     for (uint32_t i = 0; i < stages; ++i) {
         // stage i was last used in lap `lap` where i is before the ring's place, else in the lap before
-        if (i < r.s) mm_wait(bars + i, r.lap & 1, nullptr);
-        else if (r.lap > 0) mm_wait(bars + i, (r.lap - 1) & 1, nullptr);
+        if (i < r.s) mm_wait(bars + i, r.lap & 1, nullptr, kTCWaitNs);
+        else if (r.lap > 0) mm_wait(bars + i, (r.lap - 1) & 1, nullptr, kTCWaitNs);
     }
 }
 
@@ -360,6 +372,7 @@ struct MmTc {
     int split;                  // parts of k (the cluster's size)
     int kb_part;                // 128-byte blocks of k per part
     uint32_t copy_bytes;        // of a stage's two tensor copies
+    uint32_t wait_ns;           // how long a wait lasts before it gives up
     bool pair;                  // 2 neighbouring 16-bit outputs may be stored at once
 };
 
@@ -503,7 +516,7 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
                 int ct, tt;
                 mm_place(t, q.tn, q.tm, ct, tt);
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    if (r.lap > 0 && !mm_wait(&bar_empty[r.s], (r.lap - 1) & 1, vfail)) {
+                    if (r.lap > 0 && !mm_wait(&bar_empty[r.s], (r.lap - 1) & 1, vfail, q.wait_ns)) {
                         s_fail = 1;
                         break;
                     }
@@ -527,10 +540,10 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
             uint32_t n = 0;                                      // tiles done
             for (uint32_t t = t0; t < tiles; t += gridDim.x, ++n) {
                 const uint32_t a = n & 1;
-                bool ok = n < 2 || mm_wait(&bar_ae[a], (n / 2 - 1) & 1, vfail);
+                bool ok = n < 2 || mm_wait(&bar_ae[a], (n / 2 - 1) & 1, vfail, q.wait_ns);
                 const uint32_t dacc = tmem + a * NT;
                 for (int kb = kb0; ok && kb < kb1; ++kb) {
-                    ok = mm_wait(&bar_full[r.s], r.lap & 1, vfail);
+                    ok = mm_wait(&bar_full[r.s], r.lap & 1, vfail, q.wait_ns);
                     if (!ok) break;
                     tc_fence_after();
                     // descriptor addresses count 16 bytes; one MMA reads 32 bytes of k
@@ -549,8 +562,10 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
                 }
                 tc_commit(&bar_af[a]);
             }
-            // the MMAs in flight are done before tensor memory and the stages are released
+            // the MMAs in flight are done before tensor memory and the stages are released, and the
+            // last commit has arrived where the epilogue does not wait for it any more
             mm_drain(bar_empty, r, C::kStages);
+            if (n > 0) mm_wait(&bar_af[(n - 1) & 1], ((n - 1) / 2) & 1, nullptr, kTCWaitNs);
         }
         __syncwarp();
     } else {
@@ -587,7 +602,7 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
                     if (i * 32 + lane < C::kHalf) sc[i * 32 + lane] = sa_next[i];
             }
             if (t + gridDim.x < tiles) fetch(t + gridDim.x);
-            if (ok) ok = __all_sync(0xffffffffu, mm_wait(&bar_af[a], (n / 2) & 1, vfail));
+            if (ok) ok = __all_sync(0xffffffffu, mm_wait(&bar_af[a], (n / 2) & 1, vfail, q.wait_ns));
             if (!ok) {
                 if (lane == 0) s_fail = 1;
                 for (int i = lane; i < C::kHalf; i += 32) sc[i] = __int_as_float(0x7fffffff);
@@ -630,6 +645,7 @@ __global__ void __launch_bounds__(MmCfg<NT>::kThreads, MmCfg<NT>::kCtas)
     }
 
     __syncthreads();
+    if (tid == 0 && s_fail) g_mm_gave_up = 1;
     if (split > 1) {
         // every part's sums are in its shared memory; column c of the tile falls to part c % split
         cluster_sync();
@@ -695,6 +711,13 @@ cudaError_t mm_map_rows(const int8_t* rows, int64_t n, int k, int64_t ld, int bo
 // whether 2 neighbouring 16-bit outputs of a row may be stored at once
 bool pair_out(const SqMatmul& p, int out_type) { return out_type != kSqF32 && rows_aligned(p.out, 2 * p.ldo, 4); }
 
+// INSITU_SQ_WAIT_NS, read on every call: the limit of a product's waits, at most kTCWaitNs (the default)
+uint32_t mm_wait_ns() {
+    const char* v = std::getenv("INSITU_SQ_WAIT_NS");
+    if (!v || v[0] < '0' || v[0] > '9') return kTCWaitNs;
+    return (uint32_t)std::min<unsigned long long>(std::strtoull(v, nullptr, 10), kTCWaitNs);
+}
+
 template <int NT>
 cudaError_t go_tc(const SqMatmul& p, int out_type, int split, cudaStream_t st) {
     using C = MmCfg<NT>;
@@ -712,6 +735,7 @@ cudaError_t go_tc(const SqMatmul& p, int out_type, int split, cudaStream_t st) {
     q.out_type = out_type;
     q.pair = pair_out(p, out_type);
     q.copy_bytes = (uint32_t)(box_a + box_b) * kMmK;
+    q.wait_ns = mm_wait_ns();
     q.tn = (uint32_t)((p.n + kMmM - 1) / kMmM);
     q.tm = (uint32_t)((p.m + NT - 1) / NT);
     if ((int64_t)q.tn * q.tm >= int64_t(1) << 31) return cudaErrorInvalidValue;
@@ -899,6 +923,20 @@ cudaError_t sq_matmul(SqMatmul p, int out_type, void* work, cudaStream_t st) {
     if (!al_a) copied(p.a, p.m, p.lda);
     const cudaError_t e = launch_align(q, st);
     return e ? e : launch_tc(p, out_type, st);
+}
+
+// Waits for what is queued on st; whether a product on the current device has given up a wait since the last report.
+cudaError_t sq_status(bool* gave_up, cudaStream_t st) {
+    int seen = 0;
+    const int none = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(&seen, g_mm_gave_up, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+    if (!e) e = cudaStreamSynchronize(st);
+    if (!e && seen) {
+        e = cudaMemcpyToSymbolAsync(g_mm_gave_up, &none, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+        if (!e) e = cudaStreamSynchronize(st);
+    }
+    *gave_up = seen != 0;
+    return e;
 }
 
 // Floating tokens: the dot products quantise them themselves, one launch for

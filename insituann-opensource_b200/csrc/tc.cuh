@@ -1,5 +1,5 @@
 // tc.cuh -- building blocks of the tensor-core kernels (tcgen05, mbarriers,
-// bulk and tensor copies), shared by route_tc.cu and exact_tc.cu.
+// bulk and tensor copies), shared by route_tc.cu, exact_tc.cu and sq_mm.cu.
 //
 // Every wait here is bounded (kTCWaitNs of wall time, read from the global
 // timer; the polls suspend the waiting thread in between, so that waiting

@@ -46,7 +46,7 @@ EXPORTS = [
     "ivf_kernel_launches", "ivf_batch_profile", "ivf_batch_stage_ms", "ivf_u8_search_noalloc",
     "ivf_load_centroids", "ivf_assign", "ivf_build_reorder", "ivf_kmeans_update", "ivf_pq_train", "ivf_pq_encode",
     "ivf_sq_write", "ivf_sq_read", "ivf_sq_matmul", "ivf_sq_matmul_work", "ivf_sq_scores",
-    "ivf_sq_scores_work",
+    "ivf_sq_scores_work", "ivf_sq_status",
     "ivf_read_centroids", "ivf_read_assign", "ivf_read_codebook", "ivf_read_codes", "ivf_read_u8bin",
     "ivf_read_fbin", "ivf_read_gt", "ivf_write_centroids", "ivf_write_assign", "ivf_write_codebook",
     "ivf_write_codes", "ivf_pq_load_files", "ivf_pq_insert",
@@ -126,6 +126,7 @@ _SIGS = {
     "ivf_sq_matmul_work": ([vp, i64, i64, vp, i64, i64, i32], C.c_size_t),
     "ivf_sq_scores": ([vp, i32, i64, i64, vp, i64, vp, i64, i32, vp, vp, i32, i64, vp, C.c_size_t, vp], i32),
     "ivf_sq_scores_work": ([i64, vp, i64, i64, i32], C.c_size_t),
+    "ivf_sq_status": ([vp], i32),
     "ivf_read_centroids": ([C.c_char_p, vp, i64, vp, vp], i64),
     "ivf_read_assign": ([C.c_char_p, vp, i64, vp], i64),
     "ivf_read_codebook": ([C.c_char_p, vp, i64, vp, vp, vp], i64),
@@ -749,6 +750,18 @@ def _sq_call(fn, device, *args):
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
     if rc != IVF_OK:
         _sq_fail(rc)
+
+
+def sq_status(device=None):
+    """Waits for the current stream of the device and raises InsituError when a product on it (sq_matmul,
+    SQRows.scores) gave up a wait on the device since the last such report: its outputs are not valid."""
+    import torch
+
+    load_library(require_device=True)
+    device = torch.device("cuda" if device is None else device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    _sq_call(load_library().ivf_sq_status, device)
 
 
 def sq_matmul(a, a_scale, b, b_scale, bias=None, dtype=None, out=None):
