@@ -333,6 +333,8 @@ int ivf_pq_encode(const void* d_x, int x_is_u8, long long n, int d, const int* d
  *           [-L, L]; 0 where the scale is 0
  *   value = code * scale in fp32, rounded to the type it is read in
  * A group with a NaN or an infinity has that as its scale and reads as NaN.
+ * Slots of a zeroed store that no row was written to score 0 (plus the bias),
+ * above every negative score: a bias of minus infinity keeps them out.
  * No operator here has a gradient.
  *
  * Device pointers of the current device; work is queued on `stream` (a

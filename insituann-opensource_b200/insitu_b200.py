@@ -813,7 +813,8 @@ class SQRows:
 
     ``codes``  int8 [capacity, >= d] or uint8 [capacity, >= ceil(d / 2)] (two
     codes a byte, the even one in the low half); ``scales`` fp32 [capacity,
-    groups].  Slots never written are zeros.
+    groups].  Slots never written are zeros: they read as zeros and score 0 (see
+    ``scores``).
 
     Work runs on the current torch stream of the store's device; two writes of
     one store must be ordered.  No gradient flows through any call."""
@@ -937,7 +938,11 @@ class SQRows:
         8-bit store with one scale a row (group 0): x is quantised one scale a
         row as ``write`` does it, then multiplied as by sq_matmul.  bias fp32
         [capacity] or None; dtype of the scores: torch.float32 (default),
-        float16 or bfloat16."""
+        float16 or bfloat16.
+
+        A slot never written scores 0, above every negative score.  Where the
+        best rows of a store that is not full are looked for, give a bias of
+        minus infinity for its empty slots and 0 for the others."""
         import torch
 
         if self.bits != 8 or self._groups != 1:
