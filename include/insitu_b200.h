@@ -376,7 +376,8 @@ int ivf_sq_read(const void* d_codes, long long ldc, const float* d_scales, long 
  *   out[i, j] = float(sum_t a[i, t] * b[j, t]) * a_scale[i] * b_scale[j] + bias[j]
  * a [m, k], b [n, k] int8 (any value), rows lda and ldb bytes apart; scales
  * and bias (may be NULL) fp32, dense; out [m, n] of out_type, rows ldo values
- * apart.  The sum is exact (1 <= k <= IVF_SQ_MAX_K); the rest is fp32, rounded
+ * apart.  The sum is exact (1 <= k <= IVF_SQ_MAX_K); the rest is fp32 in the order
+ * written (a sum times a_scale that leaves fp32's range stays lost), rounded
  * once to out_type.  m, n < 2^31.  d_work: scratch of ivf_sq_matmul_work()
  * bytes, 16-byte aligned, for operands whose rows are not 16-byte aligned (0
  * bytes, and it may be NULL, where they are and for a few tokens).

@@ -220,7 +220,7 @@ cudaError_t pq_merge_shards(const uint64_t* adc_main, const uint64_t* exact_main
                             int nq, int k, int exact_is_int, int32_t* out_ids, float* out_dist,
                             cudaStream_t st);
 
-// ---- scalar-quantised rows (sq.cu, sq_mm.cu) -------------------------------
+// ---- scalar-quantised rows (sq_write.cu, sq_read.cu, sq_mm.cu) -------------------------------
 constexpr int kSqF32 = 0, kSqF16 = 1, kSqBF16 = 2;   // IVF_SQ_* of the C ABI
 // calls of up to this many rows look for a later row with the same slot
 // themselves (each row compares the slots after its own); longer ones go

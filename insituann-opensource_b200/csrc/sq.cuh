@@ -327,6 +327,8 @@ __device__ __noinline__ uint32_t sq_code_slow(float x, float scale) {
 // so the fused multiply-add gives it exactly: |r| < scale / 2 proves k; beyond it k
 // is one off, and on it the even neighbour is the code (both rare: one in
 // some 10^5 values).  1.5 * 2^23 is added so that the sum's last bits are k itself.
+// Where 1 / scale is infinite a zero makes r NaN; fmaxf passes over it, and `far`
+// of 0 reaches the half of 0 that such a scale has.
 template <typename T, int BITS, int E>
 __device__ __forceinline__ void sq_codes(const SqRaw<T, E>& x, const SqScale& s, uint32_t (&q)[(E * BITS + 31) / 32]) {
     constexpr float kMagic = 12582912.f;

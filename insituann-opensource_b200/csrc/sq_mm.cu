@@ -266,7 +266,6 @@ cudaError_t launch_dot(MmDot q, cudaStream_t st) {
 // g_mm_gave_up (its outputs are not valid then: what it still stores is NaN
 // mostly), lets its copies and MMAs in flight end, and returns.
 constexpr int kMmM = 128, kMmK = 128;
-constexpr int kMmMaxStages = 12;
 
 template <int NT>
 struct MmCfg {
@@ -278,8 +277,7 @@ struct MmCfg {
     static constexpr int kHalf = NT / (kEpi / 4);                 // columns of an epilogue warp
     static constexpr int kChunk = kHalf < 32 ? kHalf : 32;
     static constexpr int kStatic = kEpi * kHalf * 4 + 1024;       // static arrays
-    static constexpr int kFit = (227 * 1024 / kCtas - 1024 - 1024 - kStatic) / kStage;   // 1 KB to align, 1 KB of the system's
-    static constexpr int kStages = kFit < kMmMaxStages ? kFit : kMmMaxStages;
+    static constexpr int kStages = (227 * 1024 / kCtas - 1024 - 1024 - kStatic) / kStage;   // 1 KB to align, 1 KB of the system's
     static constexpr size_t kSmem = (size_t)kStage * kStages + 1024;
     static_assert(kStages >= 2 && (size_t)kMmM * NT * 4 <= (size_t)kStage * kStages, "a split tile's sums fit the stages");
 };

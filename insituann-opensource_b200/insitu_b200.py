@@ -772,7 +772,8 @@ def sq_matmul(a, a_scale, b, b_scale, bias=None, dtype=None, out=None):
     a int8 [m, k] and b int8 [n, k] (rows at any distance; 16-byte aligned rows
     are fastest), a_scale fp32 [m], b_scale fp32 [n], bias fp32 [n] or None.
     dtype: torch.float32 (default), float16 or bfloat16.  The sum is exact, the
-    rest fp32 and rounded once.  Runs on the current torch stream of the
+    rest fp32 in the order written (a sum times a_scale that leaves fp32's range
+    stays lost) and rounded once.  Runs on the current torch stream of the
     tensors' device; no gradient flows."""
     import torch
 
